@@ -5,7 +5,9 @@
  *   (1) paged-KV block gather / scatter between an engine's per-layer K/V page pools and the
  *       contiguous staging blocks that storage backends read and write;
  *   (2) chained 64-bit token-block hashing, a GPU-resident block index, and batched prefix /
- *       sliding-window / batch-get matching against it.
+ *       sliding-window / batch-get matching against it;
+ *   (3) a decode step over the pools of (1): rotary positions and append, attention of one new
+ *       token per sequence, eviction by accumulated attention weight.
  *
  * Every entry point names the interface of alibaba/tair-kvcache it stands in for (file:line
  * relative to that project's root).  Conventions:
@@ -920,6 +922,118 @@ KVCM_API int32_t kvcm_b200_replay_noalloc(const int64_t *d_keys, const int64_t *
                                           int64_t n_keys_total, int32_t *d_ext_hit, int32_t *d_int_hit,
                                           int32_t *d_written, int64_t *d_cache_blocks, uint32_t *d_status,
                                           kvcm_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * (3) A decode step over paged KV: what an engine computes on the pools that part (1) moves.
+ *
+ * One layer's K pool and V pool hold 16-bit floats; token row `page * page_tokens + o`, KV head h, element e is at
+ *   pool + (page * page_stride + o * token_stride + h * head_stride + e) elements,
+ * the same for both pools.  [pages, page_tokens, heads, dim] and [pages, heads, page_tokens, dim] tensors and slices
+ * of larger ones are all described this way; with head_stride = head_dim and token_stride = heads * head_dim a token
+ * row is a row of the gather / scatter entry points.  The reference moves these pools and never computes on them
+ * (kv_cache_manager/py_connector/vllm/data_transfer.py:119-217); its cache eviction ranks blocks by access
+ * (kv_cache_manager/optimizer/eviction_policy/lru.cc), the one here ranks tokens by the attention they received.
+ *
+ * Status words, when d_status is not NULL (four caller-zeroed uint32): [0] counts what was skipped because an index
+ * lay out of range, [1] keeps 1 + the largest offending token (append) or sequence (attend, evict) number.
+ * ---------------------------------------------------------------------------------------- */
+#define KVCM_DTYPE_BF16 0
+#define KVCM_DTYPE_FP16 1
+
+typedef struct kvcm_b200_kv_pools {
+    void *k_pool; /* device address of element 0; may not overlap v_pool's rows */
+    void *v_pool;
+    int64_t pool_pages;
+    int64_t page_stride; /* in elements */
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t page_tokens;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int32_t dtype; /* KVCM_DTYPE_* */
+} kvcm_b200_kv_pools_t;
+
+/* Rotary positions and append.  For token t: the first rotary_dim elements of every query and key head are rotated by
+ * the angles positions[t] * inv_freq[j], j < rotary_dim / 2 - pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) when
+ * `interleaved` - with cosine and sine multiplied by `attention_factor`; the rotated queries go to query_out, the
+ * rotated keys and the values into token row slot_idx[t] of the pools.  Slot -1 marks a padding token: nothing is
+ * written to the pools for it; any other slot outside the pool is skipped and counted.  Query and query_out may be the
+ * same memory; key and value may not overlap the pools.  Angles are formed in 64 bits and reduced to one turn before
+ * they are rounded, so positions of any magnitude an int32 holds keep their accuracy; products are formed in 32 bits
+ * and rounded once.  A slot given twice is a data race, as in scatter.
+ * d_query may be NULL with n_q_heads = 0.  Strides are in elements between tokens and between heads; elements of a head
+ * are contiguous.  position_bytes and slot_bytes say whether the index arrays hold 4- or 8-byte integers.  rotary_dim
+ * is even, 0 .. head_dim <= 1024.  Fastest when all addresses and strides are multiples of 16 bytes and rotary_dim and head_dim - rotary_dim of 16 elements;
+ * anything else is correct. */
+KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const void *d_query, int64_t q_token_stride,
+                                        int64_t q_head_stride, int32_t n_q_heads, void *d_query_out,
+                                        int64_t qo_token_stride, int64_t qo_head_stride, const void *d_key,
+                                        int64_t k_token_stride, int64_t k_head_stride, const void *d_value,
+                                        int64_t v_token_stride, int64_t v_head_stride, const void *d_positions,
+                                        int32_t position_bytes, const void *d_slot_idx, int32_t slot_bytes,
+                                        int32_t n_tokens, const float *d_inv_freq, int32_t rotary_dim,
+                                        int32_t interleaved, float attention_factor, uint32_t *d_status,
+                                        kvcm_stream_t stream);
+
+/* Attention of one new token per sequence over its paged keys and values.  Sequence b attends tokens
+ * [max(0, len - window), len), len = context_lens[b] (window 0 = all of them); token t lies in page
+ * block_table[b * table_stride + t / page_tokens].  Query head h reads KV head h / (n_q_heads / n_kv_heads):
+ *   out[b][h] = sum_t p_t V[t],  p = softmax(scale * query[b][h] . K[t])
+ * out is [batch][n_q_heads][head_dim] contiguous, of the pools' type; d_lse, when not NULL, receives the natural
+ * logarithm of the softmax sum, [batch][n_q_heads].  A sequence without tokens, and a head whose scores are all
+ * negative infinity, give zeros and an lse of negative infinity.  What lies behind a sequence's end in its last page,
+ * or on pages it does not name, never takes part, NaN included.  A length beyond table_width * page_tokens is cut to
+ * it and counted; tokens on a page outside the pool take no part, and the page is counted.
+ * d_weights, when not NULL, accumulates the attention each cached token receives:
+ *   weights_out[b][w][t] = weights[b][w][t] + sum over the query heads of KV head w of p_t     (n_weight_heads = n_kv_heads)
+ *   weights_out[b][0][t] = weights[b][0][t] + sum over all query heads of p_t                  (n_weight_heads = 1)
+ * for the attended t; other entries are left as they are.  The two may be the same memory with the same strides.
+ * Strides of both, in elements, between sequences and between heads; every row has table_width * page_tokens entries.
+ * Scores, softmax statistics, the sums and the weights are held in 32 bits; probabilities enter the product with V as
+ * two 16-bit halves, so that only the output is rounded to 16 bits.
+ * The work is cut into equal shares over the GPU's SMs wherever sequences begin and end, so one long sequence uses all
+ * of them; shares of one head are joined by a second kernel.  d_workspace holds the shares
+ * (kvcm_b200_attend_workspace_bytes, 16-byte aligned, contents irrelevant); calls that may run at the same time need
+ * separate workspaces.  Results do not depend on timing: the same inputs give the same bits.
+ * head_dim is a multiple of 8, at most 256; pool addresses and strides are multiples of 16 bytes, query addresses and
+ * strides of 4 bytes; at most 65,536 sequences and 2^30 tokens of table per sequence. */
+KVCM_API int64_t kvcm_b200_attend_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim, int64_t table_tokens, int32_t with_weights);
+KVCM_API int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_query, int64_t q_batch_stride,
+                                        int64_t q_head_stride, int32_t batch, int32_t n_q_heads,
+                                        const int32_t *d_block_table, int64_t table_stride, int32_t table_width,
+                                        const int32_t *d_context_lens, float scale, int32_t window, void *d_out,
+                                        float *d_lse, const float *d_weights, int64_t w_batch_stride,
+                                        int64_t w_head_stride, float *d_weights_out, int64_t wo_batch_stride,
+                                        int64_t wo_head_stride, int32_t n_weight_heads, void *d_workspace,
+                                        int64_t workspace_bytes, uint32_t *d_status, kvcm_stream_t stream);
+
+/* Eviction by accumulated attention weight.  For sequence b and weight head w with len = context_lens[b] slots in use,
+ * of which slot t holds the token of position positions[b][w][t] and weight weights[b][w][t]: when len > budget, the
+ * `budget` slots that rank first are kept and packed into slots [0, budget).  Ranked first are the protected slots,
+ * whose position is greater than (largest position in use) - recent; then by weight, larger first (NaN counts as the
+ * largest); among equals the lower slot.  Survivors that lie below `budget` stay where they are; those above move, in
+ * ascending order, into the freed slots below, in ascending order: K row, V row, weight and position (of KV head w, or
+ * of all heads when n_weight_heads = 1).  Attention does not depend on the order of slots, and the positions array
+ * keeps every token's age.  Slots [budget, len) get weight 0 and position -1; slots from len on are left as they are.
+ * new_lens[b] = min(len, budget).  Sequences with len <= budget keep everything.
+ * weights_out / positions_out may be the input arrays with the same strides (the usual call) or other memory, which
+ * then receives all slots below len; new_lens may not overlap context_lens.  Pages named by the kept part of two sequences at once (a shared prefix) would be
+ * packed by both: copy them first.  Pages from ceil(budget / page_tokens) on are free afterwards.  A move from or to
+ * a page outside the pool is left out and counted; weight and position move all the same.  A length beyond
+ * table_width * page_tokens is cut to it and counted.
+ * 0 <= recent <= budget, budget >= 1.  d_workspace: kvcm_b200_evict_workspace_bytes, 16-byte aligned, contents irrelevant. */
+KVCM_API int64_t kvcm_b200_evict_workspace_bytes(int32_t batch, int32_t n_weight_heads, int64_t table_tokens,
+                                                 int32_t budget);
+KVCM_API int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, const int32_t *d_block_table,
+                                       int64_t table_stride, int32_t table_width, const int32_t *d_context_lens,
+                                       int32_t budget, int32_t recent, int32_t n_weight_heads, const float *d_weights,
+                                       int64_t w_batch_stride, int64_t w_head_stride, const int32_t *d_positions,
+                                       int64_t p_batch_stride, int64_t p_head_stride, float *d_weights_out,
+                                       int64_t wo_batch_stride, int64_t wo_head_stride, int32_t *d_positions_out,
+                                       int64_t po_batch_stride, int64_t po_head_stride, int32_t *d_new_lens,
+                                       void *d_workspace, int64_t workspace_bytes, uint32_t *d_status,
+                                       kvcm_stream_t stream);
 
 #ifdef __cplusplus
 }

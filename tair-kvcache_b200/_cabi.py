@@ -29,6 +29,7 @@ STATUS_ANY = STATUS_DELETE = 0xFF
 STATUS_DELETE_KEEP_KEY = 0xFE
 VAL_STATUS_SHIFT = 33
 REPLAY_NOALLOC_MAX_KEYS = 262144
+DTYPE_BF16, DTYPE_FP16 = 0, 1  # kvcm_b200_kv_pools_t.dtype
 POLICY_LEAF_AWARE_LRU, POLICY_LRU, POLICY_RANDOM_LRU = 0, 1, 2  # kvcm_b200_replay_policy_group's per-instance policy bytes
 
 VAL_NONEMPTY = 1 << 32
@@ -58,6 +59,11 @@ class RouteExport(ctypes.Structure):
 class Iov(ctypes.Structure):
     _fields_ = [("type", ctypes.c_uint8), ("ignore", ctypes.c_uint8), ("pad_", ctypes.c_uint8 * 6), ("base", _vp),
                 ("size", _u64)]
+
+
+class KvPools(ctypes.Structure):
+    _fields_ = [("k_pool", _vp), ("v_pool", _vp), ("pool_pages", _i64), ("page_stride", _i64), ("token_stride", _i64),
+                ("head_stride", _i64), ("page_tokens", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32)]
 
 
 # name -> argtypes, in the order of include/kvcm_b200.h; every function returns int32 unless noted.
@@ -169,6 +175,14 @@ SIGNATURES = {
     "kvcm_b200_trace_replay_order": [_vp, _i64, _vp],
     "kvcm_b200_string_map_iteration_order": [_vp, _vp, _vp, _i64, _vp, _vp],
     "kvcm_b200_replay_noalloc": [_vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    "kvcm_b200_append_pages": [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32,
+                               _vp, _i32, _i32, _vp, _i32, _i32, ctypes.c_float, _vp, _vp],
+    "kvcm_b200_attend_workspace_bytes": [_i32, _i32, _i32, _i32, _i64, _i32],
+    "kvcm_b200_attend_pages": [_vp, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _vp, ctypes.c_float, _i32, _vp, _vp,
+                               _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp],
+    "kvcm_b200_evict_workspace_bytes": [_i32, _i32, _i64, _i32],
+    "kvcm_b200_evict_pages": [_vp, _i32, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                              _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp],
 }
 
 
@@ -253,3 +267,13 @@ def call_move(name, *args):
             check(fn(*[0 if a is None else int(a) for a in args]), name)
             return
     call(name, *args)
+
+
+def call_pages(name, pools, *args):
+    """A decode-step entry point by its C name; `pools` holds the fields of kvcm_b200_kv_pools_t in order and addresses
+    are integers (0 = NULL).  Through the pybind shim when it is built, else through ctypes."""
+    mod = shim()
+    if mod is not None:
+        check(getattr(mod, name[len("kvcm_b200_"):])(*pools, *args), name)
+        return
+    call(name, ctypes.addressof(KvPools(*pools)), *args)

@@ -9,7 +9,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libkvcm_b200.so")
 
 SOURCES = ["runtime.cu", "move_rows.cu", "copy_segments.cu", "hash_blocks.cu", "block_index.cu", "replay.cu",
-           "replay_lru.cu", "replay_leaf_lru.cu", "replay_random_lru.cu"]
+           "replay_lru.cu", "replay_leaf_lru.cu", "replay_random_lru.cu", "append_pages.cu", "attend_pages.cu",
+           "evict_pages.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -29,7 +30,7 @@ def sources():
 
 
 HEADERS = [os.path.join(CSRC, "kvcm_common.cuh"), os.path.join(CSRC, "replay_ids.cuh"),
-           os.path.join(CSRC, "replay_sampling.cuh"), os.path.join(CSRC, "id_table.cuh"),
+           os.path.join(CSRC, "replay_sampling.cuh"), os.path.join(CSRC, "id_table.cuh"), os.path.join(CSRC, "paged_kv.cuh"),
            os.path.join(ROOT, "include", "kvcm_b200.h")]
 OBJ_DIR = os.path.join(HERE, "build")
 
