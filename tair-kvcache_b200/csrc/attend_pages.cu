@@ -3,11 +3,15 @@
 //
 //   o_h = sum_t p_t V[t],  p = softmax_t(scale * q_h . K[t]),  t over the sequence's last `window` tokens or all.
 //
-// Bound by HBM: every K and V row is read once (512 bytes per token and KV head of 128), used by the group of query heads
-// that share the KV head, 2 to 32 multiplications per byte.  One pass with a running maximum and sum; K and V rows go
-// from HBM to shared memory by 16-byte asynchronous copies, each warp with a ring of its own, and from there by ldmatrix
-// into 16x8x16 matrix instructions whose 16 rows are the group's query heads.  A group is far too small for the 128
-// rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
+// Bound by HBM: every K and V row is read once (512 bytes per token and KV head of 128) and used by the query heads that
+// share the KV head, 2 to 32 multiplications per byte.  One pass with a running maximum and sum.
+//
+// A producer warp walks the block table and moves K and V rows into a ring of shared-memory stages with TMA tile loads -
+// boxes of up to 16 tokens by 64 elements, 128-byte swizzle - so the four consumer warps spend no instruction on
+// addresses: a first version with 16-byte asynchronous copies issued by the consumers took 670 instructions per 16
+// tokens and warp, and they, not HBM, set its pace.  A consumer takes 16 tokens of a stage: ldmatrix, 16x8x16 matrix
+// instructions whose 16 rows are the group's query heads, softmax in registers, ldmatrix, the product with V.  A group
+// is far too small for the 128 rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
 //
 // Probabilities enter the second product as two 16-bit halves, p = hi + lo, whose sum carries 16 (bf16) or more bits,
 // so the output is rounded once.  With a group of at most eight the halves cost nothing: hi takes rows 0-7 of the
@@ -17,19 +21,26 @@
 // batch are numbered through, and each of the persistent CTAs takes an equal run of them, found from the lengths on the
 // device.  A head that lies within one run is finished there; the runs of a head that is cut leave their unnormalised
 // sums and statistics in the workspace, and the second kernel joins them, in order, so results do not depend on timing.
+//
+// Every wait on an mbarrier is bounded; a CTA whose wait ran out sets status[2], waits - bounded again - for the loads it
+// has in flight, and ends, its part of the output being undefined.
+#include <cuda.h>
+
+#include <cstddef>
+
 #include "paged_kv.cuh"
 
 namespace kvcm {
 namespace {
 
-constexpr int kAttendWarps = 4;
-constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kTile = 16;                     // tokens a warp takes per step
-constexpr int kStep = kTile * kAttendWarps;   // tokens a CTA takes per step
+constexpr int kAttendWarps = 4;                            // consumers
+constexpr int kAttendThreads = (kAttendWarps + 1) * 32;    // and the producer
+constexpr int kTile = 16;                                  // tokens a consumer takes per step
+constexpr int kStep = kTile * kAttendWarps;                // tokens a CTA takes per step
+constexpr int64_t kMinRun = 4;                             // steps of a run: shorter ones are not worth joining
 constexpr int kMaxWorkers = 1024;
 constexpr int kMaxAttendHeadDim = 256;
-constexpr int kJoinThreads = 512;
-constexpr int kWeightThreads = kJoinThreads;
+constexpr int kJoinThreads = 256;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -49,6 +60,7 @@ struct AttendParams {
     int32_t n_weight_heads;
     // workspace
     int64_t *steps_before;  // [batch + 1] steps of all sequences before this one, one KV head and row tile counted
+    int4 *runs;             // [workers] where each run begins: sequence, unit, step within the unit (0: nothing is cut)
     float *part_o;          // [workers * 2][rows][dim]
     float2 *part_ml;        // [workers * 2][rows] maximum and sum of a share, the maximum in units of log2
     float2 *whole_ml;       // [batch][n_q_heads], heads that one CTA finished
@@ -59,12 +71,14 @@ struct AttendParams {
     int32_t units;      // KV heads * row tiles
     int32_t table_tokens;
     int32_t window;
+    int32_t box;  // tokens of a TMA box: the largest power of two up to 16 that divides page_tokens
     float scale_log2;
     int32_t workers;
 };
 
 struct Span {
     int32_t first, len;  // attended tokens [first, len)
+    int32_t base;        // first rounded down to a tile
     int32_t steps;
 };
 
@@ -72,23 +86,28 @@ __device__ __forceinline__ Span SpanOf(const AttendParams &p, int32_t b) {
     Span s;
     s.len = max(0, min(__ldg(p.lens + b), p.table_tokens));
     s.first = p.window > 0 ? max(0, s.len - p.window) : 0;
-    s.steps = (s.len - s.first + kStep - 1) / kStep;
+    s.base = s.first & ~(kTile - 1);
+    s.steps = (s.len - s.base + kStep - 1) / kStep;
     return s;
 }
 
-// Steps per worker, the same in both kernels.
-__device__ __forceinline__ int64_t StepsPerWorker(int64_t all, int32_t workers) {
+// Steps per run, the same in both kernels.
+__device__ __forceinline__ int64_t StepsPerRun(int64_t all, int32_t workers) {
     const int64_t per = (all + workers - 1) / workers;
-    return per > 0 ? per : 1;
+    return per > kMinRun ? per : kMinRun;
 }
 
-__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void *src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ float Exp2(float x) {  // results below 2^-126 are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
 }
-__device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void CopyWait() {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(kPending) : "memory");
+__device__ __forceinline__ void LoadBox(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t head, int32_t token,
+                                        int32_t page, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+        "l"(map), "r"(x), "r"(head), "r"(token), "r"(page), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void LoadMatrix(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
@@ -133,55 +152,90 @@ __device__ __forceinline__ void SplitPair(float p0, float p1, uint32_t &hi, uint
 }
 
 // Shapes of the main kernel: kDim (64, 128, 256) is head_dim rounded up, kRows (8, 16) the query heads of a row tile.
+// Two CTAs per SM where the ring and the joined sums leave room, with as many stages as then fit.
 template <int kDim, int kRows>
 struct AttendShape {
-    static constexpr int kRowBytes = kDim * 2;
-    static constexpr int kTileBytes = kTile * kRowBytes;  // of K, and again of V
-    static constexpr int kStages = kDim == 64 ? 4 : (kDim == 256 && kRows == 16 ? 2 : 3);
-    static constexpr int kRingBytes = kAttendWarps * kStages * 2 * kTileBytes;
-    static constexpr int kSmemBytes = kRingBytes + kAttendWarps * kRows * kDim * 4;  // + the warps' sums
-    // an SM's 228 KB, of which every CTA takes 1 KB for itself and the kernel's small arrays
-    static constexpr int kFit = 228 * 1024 / (kSmemBytes + 1024 + 640);
-    static constexpr int kCtasPerSm = kFit < 2 ? kFit : 2;
+    static constexpr int kHalves = kDim / 64;              // boxes across a row
+    static constexpr int kTileBytes = kTile * kDim * 2;    // of K, and again of V
+    static constexpr int kStageBytes = kAttendWarps * 2 * kTileBytes;
+    static constexpr int kStages = kDim == 64 ? 5 : (kRows == 16 ? 2 : 3);
+    static constexpr int kRingBytes = kStages * kStageBytes;
+    static constexpr int kCtasPerSm = kDim == 256 ? 1 : 2;
 };
 
+// What the producer tells the consumers about a step.
+struct __align__(16) StepNote {
+    int32_t b, head0, rows;  // sequence, first query head and number of query heads
+    int32_t step;            // within the unit
+    int32_t next_b, next_head0, next_rows;  // of the share that follows; set in a share's last step
+    uint32_t flags;
+    uint32_t valid[kAttendWarps];  // which of a consumer's 16 tokens take part
+};
+// Shared memory of the main kernel.  The ring comes first: swizzled tiles have to begin on a 1 KB boundary.
+template <int kDim, int kRows>
+struct __align__(1024) AttendShared {
+    using Shape = AttendShape<kDim, kRows>;
+    uint8_t ring[Shape::kRingBytes];
+    float sums[kAttendWarps][kRows][kDim];
+    float2 ml[kAttendWarps][kRows];
+    StepNote notes[Shape::kStages];
+    uint64_t full[Shape::kStages], empty[Shape::kStages], joined;
+    int64_t scan_warp[kAttendWarps + 1];
+    int64_t found_before;
+    int32_t found_b;
+    volatile uint32_t gave_up;
+};
+// What a launch asks for: the structure without its padding to a multiple of 1 KB.
+template <int kDim, int kRows>
+constexpr int AttendSmemBytes() {
+    using Shared = AttendShared<kDim, kRows>;
+    return static_cast<int>(offsetof(Shared, gave_up)) + 4;
+}
+constexpr uint32_t kShareEnds = 1, kShareWhole = 2, kShareBeginsRun = 4, kMoreFollow = 8;
+
 template <typename T, int kDim, int kRows, bool kScores>
-__global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCtasPerSm) AttendPagesKernel(const AttendParams p) {
+__global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCtasPerSm)
+    AttendPagesKernel(const AttendParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using Shape = AttendShape<kDim, kRows>;
     constexpr int kStages = Shape::kStages;
-    constexpr int kPieces = kDim / 8;               // 16-byte pieces of a row
-    constexpr int kRowsPerCopy = 32 / kPieces;      // rows one copy instruction of a warp covers
-    constexpr int kCopies = kTile / kRowsPerCopy;   // copy instructions per tile of K
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scan_warp[kAttendWarps];
-    __shared__ int64_t found_before;
-    __shared__ int32_t found_b;
-    __shared__ uint32_t valid_masks[kAttendWarps][kStages];
-    __shared__ float2 join_ml[kAttendWarps][kRows];
+    extern __shared__ __align__(1024) uint8_t smem[];
+    AttendShared<kDim, kRows> &sh = *reinterpret_cast<AttendShared<kDim, kRows> *>(smem);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float *join_o = reinterpret_cast<float *>(smem + Shape::kRingBytes);  // [warps][kRows][kDim]
+    const uint32_t ring = SmemAddr(sh.ring);
 
-    // ---- the steps of this CTA: [begin, begin + n_steps) of all steps, found by a scan over the sequences
+    // ---- the run of this CTA: steps [begin, begin + n_steps) of all, found by a scan over the sequences
     const int32_t chunk = (p.batch + kAttendThreads - 1) / kAttendThreads;
     const int32_t b_first = min(p.batch, static_cast<int32_t>(tid) * chunk), b_last = min(p.batch, b_first + chunk);
     int64_t mine = 0;
     for (int32_t b = b_first; b < b_last; ++b) mine += SpanOf(p, b).steps;
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            MbarInit(SmemAddr(&sh.full[s]), 1);
+            MbarInit(SmemAddr(&sh.empty[s]), kAttendWarps);
+        }
+        MbarInit(SmemAddr(&sh.joined), kAttendWarps);
+        sh.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.proxy.async;\n" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&v_map) : "memory");
+    }
     int64_t inclusive = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const int64_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
         if (lane >= d) inclusive += up;
     }
-    if (lane == 31) scan_warp[warp] = inclusive;
+    if (lane == 31) sh.scan_warp[warp] = inclusive;
     __syncthreads();
     int64_t before = inclusive - mine, all = 0;
 #pragma unroll
-    for (int w = 0; w < kAttendWarps; ++w) {
-        if (w < static_cast<int>(warp)) before += scan_warp[w];
-        all += scan_warp[w];
+    for (int w = 0; w <= kAttendWarps; ++w) {
+        if (w < static_cast<int>(warp)) before += sh.scan_warp[w];
+        all += sh.scan_warp[w];
     }
     const int64_t total = all * p.units;
-    const int64_t per = StepsPerWorker(total, p.workers);
+    const int64_t per = StepsPerRun(total, p.workers);
     const int64_t begin = blockIdx.x * per;
     if (blockIdx.x == 0) {  // the second kernel reads where each sequence begins
         int64_t at = before;
@@ -192,8 +246,20 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
         }
         if (tid == 0) p.steps_before[p.batch] = all;
     }
+    // Sequences without tokens belong to no run: zeros, here.
+    for (int32_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        if (SpanOf(p, b).steps != 0) continue;
+        T *out = reinterpret_cast<T *>(p.out) + static_cast<int64_t>(b) * p.n_q_heads * p.pools.head_dim;
+        for (int32_t i = tid; i < p.n_q_heads * p.pools.head_dim; i += kAttendThreads) out[i] = Half16<T>::FromFloat(0.0f);
+        if (p.lse != nullptr) {
+            for (int32_t i = tid; i < p.n_q_heads; i += kAttendThreads) p.lse[static_cast<int64_t>(b) * p.n_q_heads + i] = -INFINITY;
+        }
+    }
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    if (begin >= total) return;
+    if (begin >= total) {
+        if (tid == 0) p.runs[blockIdx.x] = make_int4(0, 0, 0, 0);
+        return;
+    }
     if (before * p.units <= begin && begin < (before + mine) * p.units) {
         int64_t at = before;
         int32_t b = b_first;
@@ -202,150 +268,223 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
             if (begin < (at + steps) * p.units) break;
             at += steps;
         }
-        found_b = b;
-        found_before = at * p.units;
+        sh.found_b = b;
+        sh.found_before = at * p.units;
     }
     __syncthreads();
     const int32_t n_steps = static_cast<int32_t>(min(per, total - begin));
+    int32_t b = sh.found_b;
+    Span span = SpanOf(p, b);
+    const int64_t inside = begin - sh.found_before;
+    int32_t unit = static_cast<int32_t>(inside / span.steps);
+    int32_t step = static_cast<int32_t>(inside - static_cast<int64_t>(unit) * span.steps);
 
-    // A place in this CTA's run of steps.
-    struct Cursor {
-        int32_t b, unit, step;
-        Span span;
-        __device__ __forceinline__ void Next(const AttendParams &p, bool more) {
-            if (++step < span.steps) return;
-            step = 0;
-            if (++unit < p.units || !more) return;
-            unit = 0;
-            do {
-                span = SpanOf(p, ++b);
-            } while (span.steps == 0);
+    // Bounded wait; when it runs out, this CTA's other waits end at their first poll.
+    auto wait = [&](uint64_t &bar, uint32_t parity) {
+        if (MbarTryWait(SmemAddr(&bar), parity)) return;
+        if (!BoundedWait(SmemAddr(&bar), parity, sh.gave_up ? 1u : kSpinLimit) && sh.gave_up == 0) {
+            sh.gave_up = 1;
+            if (p.status != nullptr) p.status[2] = 1;
         }
     };
-    Cursor now;
-    now.b = found_b;
-    now.span = SpanOf(p, now.b);
-    const int64_t inside = begin - found_before;
-    now.unit = static_cast<int32_t>(inside / now.span.steps);
-    now.step = static_cast<int32_t>(inside - static_cast<int64_t>(now.unit) * now.span.steps);
-    Cursor ahead = now;
 
-    const uint32_t ring = SmemAddr(smem) + warp * (kStages * 2 * Shape::kTileBytes);
-    const uint32_t copy_piece = lane % kPieces, copy_row = lane / kPieces;
-    const uint32_t copy_bytes = copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? 16u : 0u;
-
-    // Starts the copies of this warp's 16 tokens of step `ahead` into a stage.  Rows that take no part are filled with
-    // zeros, so that whatever lies there cannot reach a product.
-    auto fetch = [&](int stage) {
-        const int32_t kv = ahead.unit / p.row_tiles;
-        const int32_t t = ahead.span.first + ahead.step * kStep + static_cast<int32_t>(warp) * kTile +
-                          static_cast<int32_t>(lane & (kTile - 1));
-        int64_t off = -1;
-        if (t < ahead.span.len) {
-            const int32_t page_i = t / p.pools.page_tokens;
-            const int32_t within = t - page_i * p.pools.page_tokens;
-            const int64_t page = __ldg(p.table + ahead.b * p.table_stride + page_i);
-            if (page >= 0 && page < p.pools.pool_pages) {
-                off = page * p.pools.page_stride + within * p.pools.token_stride + kv * p.pools.head_stride;
-            } else if (ahead.unit == 0 && lane < kTile && (within == 0 || t == ahead.span.first)) {
-                CountSkipped(p.status, static_cast<uint32_t>(ahead.b), 1u);
+    if (warp == kAttendWarps) {
+        // ---- producer: one lane per box of `box` tokens
+        if (lane == 0) p.runs[blockIdx.x] = make_int4(b, unit, step, 0);
+        const int32_t boxes = kStep / p.box;  // 4 .. 64
+        const uint32_t box_bits = (1u << p.box) - 1u;
+        int32_t kv = unit / p.row_tiles;
+        int32_t row_tile = unit - kv * p.row_tiles;
+        int32_t share_first = step;
+        int stage = 0;
+        uint32_t parity = 1;  // the first pass over the ring finds every stage sh.empty
+        for (int32_t s = 0; s < n_steps; ++s) {
+            uint32_t valid[2];
+            int32_t page[2], token[2];
+            uint32_t issued = 0;
+            const int32_t t_step = span.base + step * kStep;
+            // table first: its latency passes while the stage is still in use
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int32_t i = r * 32 + static_cast<int32_t>(lane);
+                const int32_t t = t_step + i * p.box;
+                valid[r] = 0;
+                page[r] = -1;
+                token[r] = 0;
+                if (i < boxes && t < span.len && t + p.box > span.first) {
+                    const int32_t page_i = t / p.pools.page_tokens;
+                    token[r] = t - page_i * p.pools.page_tokens;
+                    const int32_t at = __ldg(p.table + b * p.table_stride + page_i);
+                    if (at >= 0 && at < p.pools.pool_pages) {
+                        page[r] = at;
+                        valid[r] = box_bits;
+                        if (t < span.first) valid[r] &= box_bits << (span.first - t);
+                        if (t + p.box > span.len) valid[r] &= box_bits >> (t + p.box - span.len);
+                        ++issued;
+                    } else if (unit == 0 && (token[r] == 0 || t <= span.first)) {
+                        CountSkipped(p.status, static_cast<uint32_t>(b), 1u);  // once for each page
+                    }
+                }
+            }
+            const uint32_t all_issued = __reduce_add_sync(0xffffffffu, issued);
+            // a tile's mask, from the boxes that lie in it
+            const int32_t per_tile = kTile / p.box;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                uint32_t bits = valid[r] << (((r * 32 + lane) * p.box) & (kTile - 1));
+                for (int d = 1; d < per_tile; d *= 2) bits |= __shfl_xor_sync(0xffffffffu, bits, d);
+                valid[r] = bits;
+            }
+            wait(sh.empty[stage], parity);
+            StepNote &note = sh.notes[stage];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int32_t i = r * 32 + static_cast<int32_t>(lane);
+                if (i < boxes && i % per_tile == 0) note.valid[i / per_tile] = valid[r];
+            }
+            const bool unit_ends = step + 1 == span.steps;
+            const bool share_ends = unit_ends || s + 1 == n_steps;
+            const int32_t this_b = b, this_step = step, this_kv = kv, this_tile = row_tile;
+            uint32_t flags = 0;
+            if (share_ends) {
+                flags = kShareEnds | (share_first == 0 && unit_ends ? kShareWhole : 0u) |
+                        (s == this_step - share_first ? kShareBeginsRun : 0u) | (s + 1 < n_steps ? kMoreFollow : 0u);
+            }
+            ++step;
+            if (share_ends && s + 1 < n_steps) {  // on to the next unit, or the next sequence that has tokens
+                step = share_first = 0;
+                if (++row_tile == p.row_tiles) {
+                    row_tile = 0;
+                    ++kv;
+                }
+                if (++unit == p.units) {
+                    unit = kv = 0;
+                    do {
+                        span = SpanOf(p, ++b);
+                    } while (span.steps == 0);
+                }
+            }
+            if (lane == 0) {
+                note.b = this_b;
+                note.head0 = this_kv * p.group + this_tile * kRows;
+                note.rows = min(kRows, p.group - this_tile * kRows);
+                note.step = this_step;
+                note.next_b = b;
+                note.next_head0 = kv * p.group + row_tile * kRows;
+                note.next_rows = min(kRows, p.group - row_tile * kRows);
+                note.flags = flags;
+            }
+            __syncwarp();
+            const uint32_t bar = SmemAddr(&sh.full[stage]);
+            if (lane == 0) MbarArriveExpectTx(bar, all_issued * p.box * kDim * 2 * 2);
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if (page[r] >= 0) {
+                    const uint32_t row = (r * 32 + lane) * p.box;  // within the step
+                    const uint32_t to = ring + stage * Shape::kStageBytes + (row / kTile) * 2 * Shape::kTileBytes + (row % kTile) * 128;
+#pragma unroll
+                    for (int h = 0; h < Shape::kHalves; ++h) {
+                        LoadBox(to + h * kTile * 128, &k_map, h * 64, this_kv, token[r], page[r], bar);
+                        LoadBox(to + Shape::kTileBytes + h * kTile * 128, &v_map, h * 64, this_kv, token[r], page[r], bar);
+                    }
+                }
+            }
+            if (++stage == kStages) {
+                stage = 0;
+                parity ^= 1;
             }
         }
-        const uint32_t valid = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
-        if (lane == 0) valid_masks[warp][stage] = valid;
-        const uint32_t k_to = ring + stage * 2 * Shape::kTileBytes;
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const uint32_t row = i * kRowsPerCopy + copy_row;
-            const int64_t row_off = __shfl_sync(0xffffffffu, off, row);
-            const uint32_t bytes = row_off >= 0 ? copy_bytes : 0u;
-            const int64_t from = bytes != 0 ? row_off + copy_piece * 16 : 0;
-            const uint32_t to = k_to + row * Shape::kRowBytes + ((copy_piece ^ (row & 7)) * 16);
-            CopyAsync16(to, p.pools.k + from, bytes);
-            CopyAsync16(to + Shape::kTileBytes, p.pools.v + from, bytes);
+        // nothing may arrive in shared memory that is no longer this CTA's
+        for (int s = 0; s < kStages; ++s) {
+            if (s < n_steps) wait(sh.full[s], ((n_steps - 1 - s) / kStages) & 1);
         }
-    };
+        return;
+    }
 
+    // ---- consumers
     constexpr int kOut = kDim / 8;
     float o[kOut][4];
     uint32_t qa[kDim / 16][kRows == 8 ? 2 : 4];
     float top[2], sum[2];  // of rows lane / 4 and lane / 4 + 8
-
+    auto load_queries = [&](int32_t of_b, int32_t head0, int32_t rows) {
+        const T *q = reinterpret_cast<const T *>(p.query) + of_b * p.q_batch + head0 * p.q_head;
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        if (s < n_steps) {
-            fetch(s);
-            ahead.Next(p, s + 1 < n_steps);
-        }
-        CopyCommit();
-    }
-    bool fresh = true;
-    int32_t share_first = now.step;
-    int stage = 0;
-    for (int32_t s = 0; s < n_steps; ++s) {
-        CopyWait<kStages - 2>();
-        __syncwarp();
-        if (s + kStages - 1 < n_steps) {
-            fetch(stage == 0 ? kStages - 1 : stage - 1);
-            ahead.Next(p, s + kStages < n_steps);
-        }
-        CopyCommit();
-
-        const int32_t kv = now.unit / p.row_tiles;
-        const int32_t row_tile = now.unit - kv * p.row_tiles;
-        const int32_t head0 = kv * p.group + row_tile * kRows;             // first query head of this tile
-        const int32_t rows = min(kRows, p.group - row_tile * kRows);       // query heads of this tile
-        if (fresh) {
-            fresh = false;
-            share_first = now.step;
-            const T *q = reinterpret_cast<const T *>(p.query) + now.b * p.q_batch + head0 * p.q_head;
+        for (int ks = 0; ks < kDim / 16; ++ks) {
 #pragma unroll
-            for (int ks = 0; ks < kDim / 16; ++ks) {
+            for (int half = 0; half < 2; ++half) {
+                const int col = ks * 16 + half * 8 + (lane & 3) * 2;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int col = ks * 16 + half * 8 + (lane & 3) * 2;
-#pragma unroll
-                    for (int r = 0; r < kRows / 8; ++r) {
-                        const int row = static_cast<int>(lane >> 2) + r * 8;
-                        uint32_t x = 0;
-                        if (row < rows && col < p.pools.head_dim) x = __ldg(reinterpret_cast<const uint32_t *>(q + row * p.q_head + col));
-                        qa[ks][half * (kRows / 8) + r] = x;
-                    }
+                for (int r = 0; r < kRows / 8; ++r) {
+                    const int row = static_cast<int>(lane >> 2) + r * 8;
+                    uint32_t x = 0;
+                    if (row < rows && col < p.pools.head_dim) x = __ldg(reinterpret_cast<const uint32_t *>(q + row * p.q_head + col));
+                    qa[ks][half * (kRows / 8) + r] = x;
                 }
             }
-#pragma unroll
-            for (int j = 0; j < kOut; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-            top[0] = top[1] = -INFINITY;
-            sum[0] = sum[1] = 0.0f;
         }
-
-        const uint32_t valid = valid_masks[warp][stage];
-        // where this thread's scores of row lane / 4 go: two pairs of tokens, eight apart
-        const int64_t score_at = kScores ? (static_cast<int64_t>(now.b) * p.n_q_heads + head0 + (lane >> 2)) * p.score_stride +
-                                               static_cast<int64_t>(now.step) * kStep + warp * kTile + (lane & 3) * 2
-                                         : 0;
-        if (kScores && valid == 0) {
+    };
+    auto clear = [&]() {
 #pragma unroll
-            for (int r = 0; r < kRows / 8; ++r) {
-                if (static_cast<int>(lane >> 2) + r * 8 < rows) {
-                    float *to = p.scores + score_at + r * 8 * p.score_stride;
-                    *reinterpret_cast<float2 *>(to) = make_float2(-INFINITY, -INFINITY);
-                    *reinterpret_cast<float2 *>(to + 8) = make_float2(-INFINITY, -INFINITY);
+        for (int j = 0; j < kOut; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        top[0] = top[1] = -INFINITY;
+        sum[0] = sum[1] = 0.0f;
+    };
+    {
+        const int32_t kv = unit / p.row_tiles, row_tile = unit - kv * p.row_tiles;
+        load_queries(b, kv * p.group + row_tile * kRows, min(kRows, p.group - row_tile * kRows));
+        clear();
+    }
+    // lane's row and 16-byte column in the swizzled tiles, for the K and the V product
+    const uint32_t k_row = (lane & 7) + ((lane >> 4) << 3), v_row = lane & 15;
+    const uint32_t k_lane = k_row * 128 + ((((lane >> 3) & 1) ^ (k_row & 7)) * 16);
+    const uint32_t v_lane = Shape::kTileBytes + v_row * 128 + (((lane >> 4) ^ (v_row & 7)) * 16);
+    const int32_t k_steps = (p.pools.head_dim + 15) / 16;  // 16-element pieces of a row that are not padding
+    int stage = 0;
+    uint32_t parity = 0, join_parity = 0;
+    for (int32_t s = 0; s < n_steps; ++s) {
+        wait(sh.full[stage], parity);
+        const StepNote &note = sh.notes[stage];
+        const uint32_t valid = note.valid[warp];
+        const uint32_t flags = note.flags;
+        const uint32_t tile = ring + stage * Shape::kStageBytes + warp * 2 * Shape::kTileBytes;
+        int64_t score_at = 0;  // where this thread's scores of row lane / 4 go: two pairs of tokens, eight apart
+        int32_t score_rows = 0;
+        if (kScores) {
+            score_rows = note.rows;
+            score_at = (static_cast<int64_t>(note.b) * p.n_q_heads + note.head0 + (lane >> 2)) * p.score_stride +
+                       static_cast<int64_t>(note.step) * kStep + warp * kTile + (lane & 3) * 2;
+            if (valid == 0) {
+#pragma unroll
+                for (int r = 0; r < kRows / 8; ++r) {
+                    if (static_cast<int>(lane >> 2) + r * 8 < score_rows) {
+                        float *to = p.scores + score_at + r * 8 * p.score_stride;
+                        *reinterpret_cast<float2 *>(to) = make_float2(-INFINITY, -INFINITY);
+                        *reinterpret_cast<float2 *>(to + 8) = make_float2(-INFINITY, -INFINITY);
+                    }
                 }
             }
         }
         if (valid != 0) {
+            if (valid != 0xffffu) {
+                // V rows that take no part become zeros: a probability of zero would not undo a NaN there
+                for (uint32_t row = 0; row < kTile; ++row) {
+                    if ((valid >> row) & 1u) continue;
+                    for (uint32_t c = lane; c < kDim / 8; c += 32) {
+                        const uint32_t at = tile + Shape::kTileBytes + (c >> 3) * (kTile * 128) + row * 128 + (c & 7) * 16;
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(at), "r"(0) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async;\n" ::: "memory");  // before the stage's next load
+                __syncwarp();
+            }
             // ---- scores of 16 tokens: two 16x8 products over the head dimension
-            const uint32_t k_at = ring + stage * 2 * Shape::kTileBytes;
             float c[2][2][4] = {};
-            {
-                const uint32_t row = (lane & 7) + ((lane >> 4) << 3);
-                const uint32_t row_at = k_at + row * Shape::kRowBytes;
-                const uint32_t piece = (lane >> 3) & 1;
 #pragma unroll
-                for (int ks = 0; ks < kDim / 16; ++ks) {
+            for (int ks = 0; ks < kDim / 16; ++ks) {
+                if (kDim == 64 || ks < kDim / 32 || ks < k_steps) {
                     uint32_t kb[4];
-                    LoadMatrix(kb, row_at + (((ks * 2 + piece) ^ (row & 7)) * 16));
+                    LoadMatrix(kb, ((tile + k_lane) ^ ((ks & 3) * 32)) + (ks >> 2) * (kTile * 128));
                     if constexpr (kRows == 8) {
                         MatrixMultiply<T>(c[ks & 1][0], qa[ks][0], 0u, qa[ks][1], 0u, kb[0], kb[1]);
                         MatrixMultiply<T>(c[ks & 1][1], qa[ks][0], 0u, qa[ks][1], 0u, kb[2], kb[3]);
@@ -359,16 +498,22 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t col = nt * 8 + (lane & 3) * 2 + (e & 1);
-                    const float v = (c[0][nt][e] + c[1][nt][e]) * p.scale_log2;
-                    x[nt][e] = (valid >> col) & 1u ? v : -INFINITY;
+                for (int e = 0; e < 4; ++e) x[nt][e] = (c[0][nt][e] + c[1][nt][e]) * p.scale_log2;
+            }
+            if (valid != 0xffffu) {
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t col = nt * 8 + (lane & 3) * 2 + (e & 1);
+                        if (((valid >> col) & 1u) == 0) x[nt][e] = -INFINITY;
+                    }
                 }
             }
             if (kScores) {
 #pragma unroll
                 for (int r = 0; r < kRows / 8; ++r) {
-                    if (static_cast<int>(lane >> 2) + r * 8 < rows) {
+                    if (static_cast<int>(lane >> 2) + r * 8 < score_rows) {
                         float *to = p.scores + score_at + r * 8 * p.score_stride;
                         *reinterpret_cast<float2 *>(to) = make_float2(x[0][r * 2], x[0][r * 2 + 1]);
                         *reinterpret_cast<float2 *>(to + 8) = make_float2(x[1][r * 2], x[1][r * 2 + 1]);
@@ -385,13 +530,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 m = fmaxf(m, top[r]);
                 const float use = m == -INFINITY ? 0.0f : m;  // nothing but negative infinity so far
-                scale_o[r] = exp2f(top[r] - use);
+                scale_o[r] = Exp2(top[r] - use);
                 top[r] = m;
                 float e[2][2];
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
-                    e[nt][0] = exp2f(x[nt][r * 2] - use);
-                    e[nt][1] = exp2f(x[nt][r * 2 + 1] - use);
+                    e[nt][0] = Exp2(x[nt][r * 2] - use);
+                    e[nt][1] = Exp2(x[nt][r * 2 + 1] - use);
                 }
                 sum[r] = sum[r] * scale_o[r] + ((e[0][0] + e[0][1]) + (e[1][0] + e[1][1]));
                 SplitPair<T>(e[0][0], e[0][1], pa[r], pl[r]);
@@ -412,14 +557,11 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                 }
             }
             // ---- the product with V
-            {
-                const uint32_t row = lane & 15;
-                const uint32_t row_at = k_at + Shape::kTileBytes + row * Shape::kRowBytes;
-                const uint32_t piece = lane >> 4;
 #pragma unroll
-                for (int j = 0; j < kDim / 16; ++j) {
+            for (int j = 0; j < kDim / 16; ++j) {
+                if (kDim == 64 || j < kDim / 32 || j < k_steps) {
                     uint32_t vb[4];
-                    LoadMatrixTransposed(vb, row_at + (((j * 2 + piece) ^ (row & 7)) * 16));
+                    LoadMatrixTransposed(vb, ((tile + v_lane) ^ ((j & 3) * 32)) + (j >> 2) * (kTile * 128));
                     MatrixMultiply<T>(o[2 * j], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
                     MatrixMultiply<T>(o[2 * j + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
                     if constexpr (kRows == 16) {
@@ -429,19 +571,20 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                 }
             }
         }
-        __syncwarp();  // the stage may be filled again
-        stage = stage + 1 == kStages ? 0 : stage + 1;
 
-        if (now.step + 1 == now.span.steps || s + 1 == n_steps) {
-            // ---- the share is complete: the warps' sums are joined in shared memory
-            fresh = true;
+        if (flags & kShareEnds) {
+            // ---- the share is complete: the warps' sums are sh.joined in shared memory
+            const int32_t rows = note.rows, head0 = note.head0, of_b = note.b;
+            const int32_t next_b = note.next_b, next_head0 = note.next_head0, next_rows = note.next_rows;
+            __syncwarp();
+            if (lane == 0) MbarArrive(SmemAddr(&sh.empty[stage]));
 #pragma unroll
             for (int r = 0; r < kRows / 8; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                if ((lane & 3) == 0) join_ml[warp][(lane >> 2) + r * 8] = make_float2(top[r], sum[r]);
+                if ((lane & 3) == 0) sh.ml[warp][(lane >> 2) + r * 8] = make_float2(top[r], sum[r]);
             }
-            float *mine_o = join_o + (warp * kRows + (lane >> 2)) * kDim + (lane & 3) * 2;
+            float *mine_o = &sh.sums[warp][lane >> 2][(lane & 3) * 2];
 #pragma unroll
             for (int j = 0; j < kOut; ++j) {
                 if constexpr (kRows == 8) {
@@ -451,31 +594,32 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                     *reinterpret_cast<float2 *>(mine_o + 8 * kDim + j * 8) = make_float2(o[j][2], o[j][3]);
                 }
             }
-            __syncthreads();
-            const bool whole = share_first == 0 && now.step + 1 == now.span.steps;
-            // a share that begins where the run does is the run's first; any other begins at its unit's first step
-            const bool begins_run = s + 1 - (now.step + 1 - share_first) == 0;
-            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (begins_run ? 0 : 1)) * kRows;
-            for (uint32_t i = tid; i < static_cast<uint32_t>(rows) * (kDim / 2); i += kAttendThreads) {
+            if (flags & kMoreFollow) load_queries(next_b, next_head0, next_rows);  // on its way while the sums are sh.joined
+            __syncwarp();
+            if (lane == 0) MbarArrive(SmemAddr(&sh.joined));
+            wait(sh.joined, join_parity);
+            join_parity ^= 1;
+            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + ((flags & kShareBeginsRun) ? 0 : 1)) * kRows;
+            for (uint32_t i = tid; i < static_cast<uint32_t>(rows) * (kDim / 2); i += kAttendWarps * 32) {
                 const uint32_t row = i / (kDim / 2);
                 const uint32_t d = (i - row * (kDim / 2)) * 2;
                 float m = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, join_ml[w][row].x);
+                for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, sh.ml[w][row].x);
                 float l = 0.0f;
                 float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kAttendWarps; ++w) {
-                    const float2 ml = join_ml[w][row];
-                    const float f = exp2f(ml.x - (m == -INFINITY ? 0.0f : m));
-                    const float2 part = *reinterpret_cast<const float2 *>(join_o + (w * kRows + row) * kDim + d);
+                    const float2 ml = sh.ml[w][row];
+                    const float f = Exp2(ml.x - (m == -INFINITY ? 0.0f : m));
+                    const float2 part = *reinterpret_cast<const float2 *>(&sh.sums[w][row][d]);
                     l += ml.y * f;
                     acc.x += part.x * f;
                     acc.y += part.y * f;
                 }
-                if (whole) {
+                if (flags & kShareWhole) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const int64_t head_at = static_cast<int64_t>(now.b) * p.n_q_heads + head0 + row;
+                    const int64_t head_at = static_cast<int64_t>(of_b) * p.n_q_heads + head0 + row;
                     if (d < static_cast<uint32_t>(p.pools.head_dim)) {
                         T *to = reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim + d;
                         *reinterpret_cast<typename Half16<T>::Pair *>(to) = Half16<T>::FromFloat2(acc.x * inv, acc.y * inv);
@@ -489,157 +633,215 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                     if (d == 0) p.part_ml[slot + row] = make_float2(m, l);
                 }
             }
-            __syncthreads();
+            __syncwarp();
+            if (lane == 0) MbarArrive(SmemAddr(&sh.joined));
+            wait(sh.joined, join_parity);  // the sums may be overwritten
+            join_parity ^= 1;
+            clear();
+        } else {
+            __syncwarp();
+            if (lane == 0) MbarArrive(SmemAddr(&sh.empty[stage]));
         }
-        now.Next(p, s + 1 < n_steps);
+        if (++stage == kStages) {
+            stage = 0;
+            parity ^= 1;
+        }
     }
-    CopyWait<0>();
 }
 
-// Where the shares of a unit lie: workers [first, last]; share w is in slot 2 w + (its unit begins within the run).
+// Where the shares of a unit lie: runs [first, last]; the share of run w is in slot 2 w + (the unit begins within the run).
 struct Shares {
     int64_t t0, per;
     int32_t first, last;
     __device__ __forceinline__ int64_t Slot(int32_t w) const { return 2 * static_cast<int64_t>(w) + (t0 > w * per ? 1 : 0); }
 };
 
-__device__ __forceinline__ Shares SharesOf(const AttendParams &p, int64_t before, int64_t steps, int64_t per, int32_t unit) {
+__device__ __forceinline__ Shares SharesAt(int64_t t0, int64_t steps, int64_t per) {
     Shares s;
-    s.t0 = before * p.units + unit * steps;
+    s.t0 = t0;
     s.per = per;
-    s.first = static_cast<int32_t>(s.t0 / per);
-    s.last = static_cast<int32_t>((s.t0 + steps - 1) / per);
+    s.first = static_cast<int32_t>(t0 / per);
+    s.last = static_cast<int32_t>((t0 + steps - 1) / per);
     return s;
 }
 
-// Joins the shares of heads that were cut, writes zeros for sequences without tokens, and, in the blocks behind those,
-// adds the attention every token received to its weight.  One block per query head, then kWeightThreads tokens of one
-// weight head per block.
+// A sum in progress: maximum (log2 units), sum of exponentials, four output elements.
+struct Partial {
+    float m, l;
+    float4 o;
+    __device__ __forceinline__ void Add(float m2, float l2, float4 o2) {
+        const float grown = fmaxf(m, m2);
+        const float use = grown == -INFINITY ? 0.0f : grown;
+        const float f = Exp2(m - use), f2 = Exp2(m2 - use);
+        l = l * f + l2 * f2;
+        o.x = o.x * f + o2.x * f2;
+        o.y = o.y * f + o2.y * f2;
+        o.z = o.z * f + o2.z * f2;
+        o.w = o.w * f + o2.w * f2;
+        m = grown;
+    }
+};
+
+// Joins the shares of heads that were cut and, in the blocks behind those, adds the attention every token received to its
+// weight.
+//
+// Join: block w looks at the point where run w begins.  When that lies within a unit, the unit's shares are joined by
+// the blocks of all such points together: with c cuts each block takes a c-th of the unit's output elements, four to a
+// thread group, over all shares, so that one long head is joined by as many blocks as computed it.
+//
+// Weights: the steps of all sequences and weight heads are cut into equal runs again.
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendParams p, uint32_t join_blocks, uint32_t weight_chunks) {
+__global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendParams p, int32_t weight_blocks) {
+    __shared__ Partial partials[kJoinThreads / 32];
+    __shared__ int32_t found_b;
+    extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count for a weight head
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const int64_t total = p.steps_before[p.batch] * p.units;
-    const int64_t per = StepsPerWorker(total, p.workers);
-    const uint32_t tid = threadIdx.x;
-    if (blockIdx.x < join_blocks) {
-        constexpr int kLanes = kDim / 2;                      // threads across a head, two elements each
-        constexpr int kParts = kJoinThreads / kLanes;         // shares summed side by side
-        __shared__ float2 sums[kParts][kLanes];
-        __shared__ float part_l[kParts];
-        const int32_t b = blockIdx.x / p.n_q_heads, head = blockIdx.x - b * p.n_q_heads;
-        const int64_t head_at = static_cast<int64_t>(b) * p.n_q_heads + head;
-        T *out = reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim;
-        const int64_t before = p.steps_before[b], steps = p.steps_before[b + 1] - before;
-        if (steps == 0) {
-            for (uint32_t d = tid; d < static_cast<uint32_t>(p.pools.head_dim); d += kJoinThreads) out[d] = Half16<T>::FromFloat(0.0f);
-            if (tid == 0 && p.lse != nullptr) p.lse[head_at] = -INFINITY;
-            return;
-        }
-        const int32_t kv = head / p.group, in_group = head - kv * p.group;
-        const int32_t row = in_group % kRows;
-        const Shares sh = SharesOf(p, before, steps, per, kv * p.row_tiles + in_group / kRows);
-        if (sh.first == sh.last) return;  // finished by the CTA that had it whole
-        __shared__ float warp_max[kJoinThreads / 32];
-        float m = -INFINITY;
-        for (int32_t w = sh.first + tid; w <= sh.last; w += kJoinThreads) m = fmaxf(m, p.part_ml[sh.Slot(w) * kRows + row].x);
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        if ((tid & 31) == 0) warp_max[tid >> 5] = m;
-        __syncthreads();
-        m = warp_max[0];
-        for (int w = 1; w < kJoinThreads / 32; ++w) m = fmaxf(m, warp_max[w]);
-        const float use = m == -INFINITY ? 0.0f : m;
-        const uint32_t part = tid / kLanes, at = tid % kLanes;
-        float2 acc = make_float2(0.0f, 0.0f);
-        float l = 0.0f;
+    const int64_t all = p.steps_before[p.batch];
+    const int64_t per = StepsPerRun(all * p.units, p.workers);
+    if (blockIdx.x < static_cast<uint32_t>(p.workers)) {
+        const int32_t w = blockIdx.x;
+        const int4 run = p.runs[w];
+        if (run.z == 0) return;
+        const int64_t steps = p.steps_before[run.x + 1] - p.steps_before[run.x];
+        const Shares sh = SharesAt(w * per - run.z, steps, per);
+        const int32_t cuts = sh.last - sh.first, cut = w - sh.first - 1;
+        const int32_t kv = run.y / p.row_tiles, row_tile = run.y - kv * p.row_tiles;
+        const int32_t rows = min(kRows, p.group - row_tile * kRows);
+        const int64_t head0 = static_cast<int64_t>(run.x) * p.n_q_heads + kv * p.group + row_tile * kRows;
+        const int32_t fours = rows * (kDim / 4);                   // groups of four output elements
+        const int32_t mine = (fours + cuts - 1) / cuts;            // this block's
+        int32_t lanes = 1;                                         // thread groups per pass, a power of two
+        while (lanes < mine && lanes < kJoinThreads) lanes *= 2;
+        const int32_t parts = kJoinThreads / lanes;                // threads that share a group's shares
+        const int32_t at = tid / parts, part = tid % parts;
+        for (int32_t base = 0; base < mine; base += lanes) {
+            const int32_t four = cut * mine + base + at;
+            const bool live = base + at < mine && four < fours;
+            const int32_t row = live ? four / (kDim / 4) : 0, d = live ? (four - row * (kDim / 4)) * 4 : 0;
+            Partial acc = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+            if (live) {
 #pragma unroll 4
-        for (int32_t w = sh.first + part; w <= sh.last; w += kParts) {
-            const int64_t slot = sh.Slot(w) * kRows + row;
-            const float2 ml = p.part_ml[slot];
-            const float2 v = *reinterpret_cast<const float2 *>(p.part_o + slot * kDim + at * 2);
-            const float f = exp2f(ml.x - use);
-            l += ml.y * f;
-            acc.x += v.x * f;
-            acc.y += v.y * f;
-        }
-        sums[part][at] = acc;
-        if (at == 0) part_l[part] = l;
-        __syncthreads();
-        if (part == 0) {
-            l = 0.0f;
-            acc = make_float2(0.0f, 0.0f);
-            for (int i = 0; i < kParts; ++i) {
-                l += part_l[i];
-                acc.x += sums[i][at].x;
-                acc.y += sums[i][at].y;
+                for (int32_t i = sh.first + part; i <= sh.last; i += parts) {
+                    const int64_t slot = sh.Slot(i) * kRows + row;
+                    const float2 ml = __ldcg(p.part_ml + slot);
+                    acc.Add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d)));
+                }
             }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (at * 2 < static_cast<uint32_t>(p.pools.head_dim)) {
-                *reinterpret_cast<typename Half16<T>::Pair *>(out + at * 2) = Half16<T>::FromFloat2(acc.x * inv, acc.y * inv);
+            for (int32_t i = 1; i < min(parts, 32); i *= 2) {
+                Partial other;
+                other.m = __shfl_xor_sync(0xffffffffu, acc.m, i);
+                other.l = __shfl_xor_sync(0xffffffffu, acc.l, i);
+                other.o.x = __shfl_xor_sync(0xffffffffu, acc.o.x, i);
+                other.o.y = __shfl_xor_sync(0xffffffffu, acc.o.y, i);
+                other.o.z = __shfl_xor_sync(0xffffffffu, acc.o.z, i);
+                other.o.w = __shfl_xor_sync(0xffffffffu, acc.o.w, i);
+                acc.Add(other.m, other.l, other.o);
             }
-            if (at == 0 && p.lse != nullptr) p.lse[head_at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+            if (parts > 32) {
+                __syncthreads();
+                if (lane == 0) partials[warp] = acc;
+                __syncthreads();
+                if (part == 0) {
+                    for (int32_t i = 1; i < parts / 32; ++i) {
+                        const Partial other = partials[warp + i];
+                        acc.Add(other.m, other.l, other.o);
+                    }
+                }
+            }
+            if (live && part == 0) {
+                const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
+                if (d < p.pools.head_dim) {  // head_dim is a multiple of eight
+                    auto *to = reinterpret_cast<typename Half16<T>::Pair *>(reinterpret_cast<T *>(p.out) + (head0 + row) * p.pools.head_dim + d);
+                    to[0] = Half16<T>::FromFloat2(acc.o.x * inv, acc.o.y * inv);
+                    to[1] = Half16<T>::FromFloat2(acc.o.z * inv, acc.o.w * inv);
+                }
+                if (d == 0 && p.lse != nullptr) p.lse[head0 + row] = acc.l == 0.0f ? -INFINITY : acc.m * kLn2 + logf(acc.l);
+            }
         }
         return;
     }
-    // ---- weights
-    extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count here
-    const uint32_t block = blockIdx.x - join_blocks;
-    const uint32_t pair = block / weight_chunks;
-    const uint32_t chunk = block - pair * weight_chunks;
-    const int32_t b = pair / p.n_weight_heads, wh = pair - b * p.n_weight_heads;
-    const Span span = SpanOf(p, b);
-    const int32_t from = span.first + static_cast<int32_t>(chunk) * kWeightThreads;
-    if (from >= span.len) return;
-    const int32_t n_heads = p.n_weight_heads == 1 ? p.n_q_heads : p.group;
-    const int32_t head0 = p.n_weight_heads == 1 ? 0 : wh * p.group;
-    const int64_t before = p.steps_before[b];
-    for (int32_t i = tid >> 5; i < n_heads; i += kWeightThreads / 32) {
-        const int32_t head = head0 + i;
-        const int32_t kv = head / p.group, in_group = head - kv * p.group;
-        const Shares sh = SharesOf(p, before, span.steps, per, kv * p.row_tiles + in_group / kRows);
-        float m, l = 0.0f;
-        if (sh.first == sh.last) {
-            const float2 ml = p.whole_ml[static_cast<int64_t>(b) * p.n_q_heads + head];
-            m = ml.x;
-            l = ml.y;
-        } else {
-            m = -INFINITY;
-            for (int32_t w = sh.first + (tid & 31); w <= sh.last; w += 32) {
-                const float2 ml = p.part_ml[sh.Slot(w) * kRows + in_group % kRows];
-                const float grown = fmaxf(m, ml.x);
-                const float use = grown == -INFINITY ? 0.0f : grown;
-                l = l * exp2f(m - use) + ml.y * exp2f(ml.x - use);
-                m = grown;
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
-                const float grown = fmaxf(m, m2);
-                const float use = grown == -INFINITY ? 0.0f : grown;
-                l = l * exp2f(m - use) + l2 * exp2f(m2 - use);
-                m = grown;
-            }
-        }
-        if ((tid & 31) == 0) head_ml[i] = make_float2(m == -INFINITY ? 0.0f : m, l == 0.0f ? 0.0f : 1.0f / l);
+
+    // ---- weights: steps [at, end) of the batch's steps times weight heads
+    const int32_t block = blockIdx.x - p.workers;
+    const int64_t total = all * p.n_weight_heads;
+    const int64_t share = (total + weight_blocks - 1) / weight_blocks;
+    int64_t at = block * share;
+    const int64_t end = min(total, at + share);
+    if (at >= end) return;
+    for (int32_t b = tid; b < p.batch; b += kJoinThreads) {
+        if (p.steps_before[b] * p.n_weight_heads <= at && at < p.steps_before[b + 1] * p.n_weight_heads) found_b = b;
     }
     __syncthreads();
-    const int32_t t = from + static_cast<int32_t>(tid);
-    if (t >= span.len) return;
-    // a token on a page outside the pool was masked like any other: its score is negative infinity
-    const float *scores = p.scores + (static_cast<int64_t>(b) * p.n_q_heads + head0) * p.score_stride + (t - span.first);
-    float received = 0.0f;
+    int32_t b = found_b;
+    const int32_t n_heads = p.n_weight_heads == 1 ? p.n_q_heads : p.group;
+    while (at < end) {
+        const Span span = SpanOf(p, b);
+        if (span.steps == 0) {
+            ++b;
+            continue;
+        }
+        const int64_t before = p.steps_before[b];
+        const int64_t inside = at - before * p.n_weight_heads;
+        const int32_t wh = static_cast<int32_t>(inside / span.steps);
+        const int32_t step0 = static_cast<int32_t>(inside - static_cast<int64_t>(wh) * span.steps);
+        const int32_t steps = static_cast<int32_t>(min(static_cast<int64_t>(span.steps - step0), end - at));
+        const int32_t head0 = p.n_weight_heads == 1 ? 0 : wh * p.group;
+        __syncthreads();
+        for (int32_t i = warp; i < n_heads; i += kJoinThreads / 32) {
+            const int32_t head = head0 + i;
+            const int32_t kv = head / p.group, in_group = head - kv * p.group;
+            const int64_t unit = static_cast<int64_t>(kv) * p.row_tiles + in_group / kRows;
+            const Shares sh = SharesAt(before * p.units + unit * span.steps, span.steps, per);
+            float m = -INFINITY, l = 0.0f;
+            if (sh.first == sh.last) {
+                const float2 ml = p.whole_ml[static_cast<int64_t>(b) * p.n_q_heads + head];
+                m = ml.x;
+                l = ml.y;
+            } else {
+                for (int32_t w = sh.first + lane; w <= sh.last; w += 32) {
+                    const float2 ml = __ldcg(p.part_ml + sh.Slot(w) * kRows + in_group % kRows);
+                    const float grown = fmaxf(m, ml.x);
+                    const float use = grown == -INFINITY ? 0.0f : grown;
+                    l = l * Exp2(m - use) + ml.y * Exp2(ml.x - use);
+                    m = grown;
+                }
+#pragma unroll
+                for (int d = 16; d > 0; d /= 2) {
+                    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
+                    const float grown = fmaxf(m, m2);
+                    const float use = grown == -INFINITY ? 0.0f : grown;
+                    l = l * Exp2(m - use) + l2 * Exp2(m2 - use);
+                    m = grown;
+                }
+            }
+            if (lane == 0) head_ml[i] = make_float2(m == -INFINITY ? 0.0f : m, l == 0.0f ? 0.0f : 1.0f / l);
+        }
+        __syncthreads();
+        // a token on a page outside the pool was masked like any other: its score is negative infinity
+        const float *scores = p.scores + (static_cast<int64_t>(b) * p.n_q_heads + head0) * p.score_stride;
+        const float *w_in = p.weights + b * p.w_batch + wh * p.w_head;
+        float *w_out = p.weights_out + b * p.wo_batch + wh * p.wo_head;
+        const int32_t last = min((step0 + steps) * kStep, span.len - span.base);  // relative to the span's base
+        for (int32_t t = step0 * kStep + static_cast<int32_t>(tid); t < last; t += kJoinThreads) {
+            if (span.base + t < span.first) continue;
+            float received = 0.0f;
 #pragma unroll 4
-    for (int32_t i = 0; i < n_heads; ++i) {
-        const float2 ml = head_ml[i];
-        received += exp2f(scores[i * p.score_stride] - ml.x) * ml.y;
+            for (int32_t i = 0; i < n_heads; ++i) {
+                const float2 ml = head_ml[i];
+                received += Exp2(__ldcg(scores + i * p.score_stride + t) - ml.x) * ml.y;
+            }
+            w_out[span.base + t] = w_in[span.base + t] + received;
+        }
+        at += steps;
+        if (at == (before + span.steps) * p.n_weight_heads) ++b;
     }
-    p.weights_out[b * p.wo_batch + wh * p.wo_head + t] = p.weights[b * p.w_batch + wh * p.w_head + t] + received;
 }
 
 int64_t Aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 struct AttendWorkspace {
-    int64_t steps_before, part_o, part_ml, whole_ml, scores, total;
+    int64_t steps_before, runs, part_o, part_ml, whole_ml, scores, total;
     int64_t score_stride;
 };
 
@@ -648,29 +850,69 @@ AttendWorkspace LayOut(int32_t batch, int32_t n_q_heads, int32_t group, int32_t 
     const int dim = head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256);
     AttendWorkspace w;
     w.steps_before = 0;
-    w.part_o = Aligned((static_cast<int64_t>(batch) + 1) * 8);
+    w.runs = Aligned((static_cast<int64_t>(batch) + 1) * 8);
+    w.part_o = w.runs + Aligned(int64_t{kMaxWorkers} * 16);
     w.part_ml = w.part_o + Aligned(int64_t{kMaxWorkers} * 2 * rows * dim * 4);
     w.whole_ml = w.part_ml + Aligned(int64_t{kMaxWorkers} * 2 * rows * 8);
     w.scores = w.whole_ml + (with_weights ? Aligned(static_cast<int64_t>(batch) * n_q_heads * 8) : 0);
-    w.score_stride = (table_tokens + kStep - 1) / kStep * kStep;
+    w.score_stride = (table_tokens + kStep - 1) / kStep * kStep + kStep;  // a window may begin within a tile
     w.total = w.scores + (with_weights ? Aligned(static_cast<int64_t>(batch) * n_q_heads * w.score_stride * 4) : 0);
     return w;
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder of tensor maps, looked up once.
+EncodeTiled GetEncodeTiled() {
+    static const EncodeTiled fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// One pool as a tensor of [page][token][head][element]; a box is `box` tokens of one head by 64 elements, elements
+// behind head_dim read as zeros.
+bool MapPool(const AttendParams &p, uint8_t *pool, bool bf16, CUtensorMap *map) {
+    const EncodeTiled encode = GetEncodeTiled();
+    if (encode == nullptr) return false;
+    // the stride of an axis of length one is not used, but has to be well-formed
+    auto stride = [](int64_t bytes, int64_t length) { return static_cast<cuuint64_t>(length > 1 ? bytes : 16); };
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.pools.head_dim), static_cast<cuuint64_t>(p.pools.n_kv_heads),
+                                static_cast<cuuint64_t>(p.pools.page_tokens), static_cast<cuuint64_t>(p.pools.pool_pages)};
+    const cuuint64_t strides[3] = {stride(p.pools.head_stride, p.pools.n_kv_heads),
+                                   stride(p.pools.token_stride, p.pools.page_tokens),
+                                   stride(p.pools.page_stride, p.pools.pool_pages)};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(p.box), 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, pool, dims, strides, box,
+                  steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int kDim, int kRows, bool kScores>
-void LaunchAttend(AttendParams p, cudaStream_t stream) {
+void LaunchAttend(AttendParams p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t stream) {
     using Shape = AttendShape<kDim, kRows>;
+    static_assert((AttendSmemBytes<kDim, kRows>() + 1024) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
     auto *main_kernel = AttendPagesKernel<T, kDim, kRows, kScores>;
     auto *join_kernel = JoinSharesKernel<T, kDim, kRows>;
-    EnsureDynamicSmem(main_kernel, Shape::kSmemBytes);
-    p.workers = std::min(kMaxWorkers, GetDeviceInfo().sm_count * Shape::kCtasPerSm);
-    main_kernel<<<p.workers, kAttendThreads, Shape::kSmemBytes, stream>>>(p);
+    EnsureDynamicSmem(main_kernel, AttendSmemBytes<kDim, kRows>());
+    const int32_t sm_count = GetDeviceInfo().sm_count;
+    p.workers = std::min(kMaxWorkers, sm_count * Shape::kCtasPerSm);
+    main_kernel<<<p.workers, kAttendThreads, AttendSmemBytes<kDim, kRows>(), stream>>>(p, k_map, v_map);
 
-    const uint32_t join_blocks = static_cast<uint32_t>(p.batch) * p.n_q_heads;
-    const int64_t most = p.window > 0 ? std::min(p.window, p.table_tokens) : p.table_tokens;
-    const uint32_t weight_chunks = kScores ? static_cast<uint32_t>((most + kWeightThreads - 1) / kWeightThreads) : 0;
+    // The second kernel's blocks wait on the device for the first kernel's end, their launch overlaps it.
+    const int32_t weight_blocks = kScores ? 2 * sm_count : 0;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(join_blocks + weight_chunks * static_cast<uint32_t>(p.batch) * p.n_weight_heads);
+    cfg.gridDim = dim3(p.workers + weight_blocks);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = kScores ? static_cast<size_t>(p.n_weight_heads == 1 ? p.n_q_heads : p.group) * 8 : 0;
     cfg.stream = stream;
@@ -679,26 +921,26 @@ void LaunchAttend(AttendParams p, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, join_kernel, p, join_blocks, std::max(weight_chunks, 1u));
+    cudaLaunchKernelEx(&cfg, join_kernel, p, weight_blocks);
 }
 
 template <typename T, int kDim>
-void DispatchAttend(const AttendParams &p, cudaStream_t stream) {
+void DispatchAttend(const AttendParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t stream) {
     if (p.group <= 8) {
-        p.scores != nullptr ? LaunchAttend<T, kDim, 8, true>(p, stream) : LaunchAttend<T, kDim, 8, false>(p, stream);
+        p.scores != nullptr ? LaunchAttend<T, kDim, 8, true>(p, k, v, stream) : LaunchAttend<T, kDim, 8, false>(p, k, v, stream);
     } else {
-        p.scores != nullptr ? LaunchAttend<T, kDim, 16, true>(p, stream) : LaunchAttend<T, kDim, 16, false>(p, stream);
+        p.scores != nullptr ? LaunchAttend<T, kDim, 16, true>(p, k, v, stream) : LaunchAttend<T, kDim, 16, false>(p, k, v, stream);
     }
 }
 
 template <typename T>
-void DispatchAttend(const AttendParams &p, cudaStream_t stream) {
+void DispatchAttend(const AttendParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t stream) {
     if (p.pools.head_dim <= 64) {
-        DispatchAttend<T, 64>(p, stream);
+        DispatchAttend<T, 64>(p, k, v, stream);
     } else if (p.pools.head_dim <= 128) {
-        DispatchAttend<T, 128>(p, stream);
+        DispatchAttend<T, 128>(p, k, v, stream);
     } else {
-        DispatchAttend<T, 256>(p, stream);
+        DispatchAttend<T, 256>(p, k, v, stream);
     }
 }
 
@@ -734,10 +976,7 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
         (with_weights && d_weights == d_weights_out && (w_batch_stride != wo_batch_stride || w_head_stride != wo_head_stride))) {
         return KVCM_ER_INVALID_PARAMS;
     }
-    const int64_t weight_blocks = with_weights ? (table_tokens / kWeightThreads + 1) * batch * n_weight_heads : 0;
-    if (batch > 65536 || n_q_heads > 4096 || table_tokens > kMaxTableTokens || weight_blocks > (int64_t{1} << 30)) {
-        return KVCM_EC_OUT_OF_LIMIT;
-    }
+    if (batch > 65536 || n_q_heads > 4096 || table_tokens > kMaxTableTokens) return KVCM_EC_OUT_OF_LIMIT;
     if ((batch > 0 && (d_query == nullptr || (d_block_table == nullptr && table_width > 0) || d_context_lens == nullptr ||
                        d_out == nullptr || d_workspace == nullptr)) ||
         !RowsAre16ByteAligned(*pools) || (reinterpret_cast<uintptr_t>(d_workspace) & 15u) != 0 ||
@@ -770,6 +1009,7 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.wo_head = wo_head_stride;
     p.n_weight_heads = with_weights ? n_weight_heads : 0;
     p.steps_before = reinterpret_cast<int64_t *>(ws + w.steps_before);
+    p.runs = reinterpret_cast<int4 *>(ws + w.runs);
     p.part_o = reinterpret_cast<float *>(ws + w.part_o);
     p.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml);
     p.whole_ml = reinterpret_cast<float2 *>(ws + w.whole_ml);
@@ -784,10 +1024,15 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.table_tokens = static_cast<int32_t>(table_tokens);
     p.window = window;
     p.scale_log2 = scale * kLog2e;
-    if (pools->dtype == KVCM_DTYPE_BF16) {
-        DispatchAttend<__nv_bfloat16>(p, AsStream(stream));
+    p.box = kTile;
+    while (pools->page_tokens % p.box != 0) p.box /= 2;
+    const bool bf16 = pools->dtype == KVCM_DTYPE_BF16;
+    CUtensorMap k_map, v_map;
+    if (!MapPool(p, p.pools.k, bf16, &k_map) || !MapPool(p, p.pools.v, bf16, &v_map)) return KVCM_ER_CUDAMEMCPY_ERROR;
+    if (bf16) {
+        DispatchAttend<__nv_bfloat16>(p, k_map, v_map, AsStream(stream));
     } else {
-        DispatchAttend<__half>(p, AsStream(stream));
+        DispatchAttend<__half>(p, k_map, v_map, AsStream(stream));
     }
     return LaunchStatus();
 }

@@ -218,6 +218,10 @@ def _check_attend(q, k_pool, v_pool, table, lens, dtype, window=0, scale=None, *
     ([9000], 8, 1, 128, 32, "nhd", 0),                          # one sequence over many CTAs
     ([40] * 70 + [700] * 3, 8, 4, 64, 16, "nhd", 0),            # many sequences per CTA
     ([5] * 300, 2, 1, 32, 16, "nhd", 0),                        # more sequences than a CTA has threads
+    ([77, 150], 4, 2, 64, 4, "nhd", 0),                         # four, two and one tokens to a TMA box
+    ([77, 150], 4, 2, 128, 2, "hnd", 20),
+    ([333], 4, 2, 136, 1, "nhd", 0),
+    ([333, 70], 4, 2, 200, 12, "nhd", 69),
 ])
 def test_attend_matches_the_definition(lens, hq, hkv, dim, page, layout, window, dtype):
     case = _attend_case(sum(lens) + dim, lens, hq, hkv, dim, dtype, page, layout)
