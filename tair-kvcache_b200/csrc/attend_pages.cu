@@ -6,39 +6,32 @@
 // Bound by HBM: every K and V row is read once (512 bytes per token and KV head of 128) and used by the query heads that
 // share the KV head, 2 to 32 multiplications per byte.  One pass with a running maximum and sum.
 //
-// A producer warp walks the block table and moves K and V rows into a ring of shared-memory stages with TMA tile loads -
-// boxes of up to 16 tokens by 64 elements, 128-byte swizzle - so the four consumer warps spend no instruction on
-// addresses: a first version with 16-byte asynchronous copies issued by the consumers took 670 instructions per 16
-// tokens and warp, and they, not HBM, set its pace.  A consumer takes 16 tokens of a stage: ldmatrix, 16x8x16 matrix
-// instructions whose 16 rows are the group's query heads, softmax in registers, ldmatrix, the product with V.  A group
-// is far too small for the 128 rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
+// Four warps to a CTA, each with a ring of its own: tiles of 16 tokens of one KV head come from HBM by 16-byte asynchronous
+// copies, issued by the warp two tiles ahead, the table entry of the one after those already on its way; then
+// ldmatrix, 16x8x16 matrix instructions whose 16 rows are the group's query heads, softmax in registers, and the product
+// with V.  No warp waits for another until a head is complete.  (TMA tile loads were measured in two forms and left:
+// with a producer warp for the CTA, 65 cycles to issue each box set the pace, 1050 to 1700 for a step of four tiles; with
+// every warp loading its own tile, the four barrier operations a tile needs, about 100 cycles each, did.)  A group is
+// far too small for the 128 rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
 //
 // Probabilities enter the second product as two 16-bit halves, p = hi + lo, whose sum carries 16 (bf16) or more bits,
 // so the output is rounded once.  With a group of at most eight the halves cost nothing: hi takes rows 0-7 of the
 // matrix instruction, lo the rows 8-15 that the group leaves free.
 //
-// The work is cut by tokens, not by sequences: the steps (kStep tokens of one KV head of one sequence) of the whole
+// The work is cut by tokens, not by sequences: the steps (four tiles of one sequence) of the whole
 // batch are numbered through, and each of the persistent CTAs takes an equal run of them, found from the lengths on the
 // device.  A head that lies within one run is finished there; the runs of a head that is cut leave their unnormalised
 // sums and statistics in the workspace, and the second kernel joins them, in order, so results do not depend on timing.
-//
-// Every wait on an mbarrier is bounded; a CTA whose wait ran out sets status[2], waits - bounded again - for the loads it
-// has in flight, and ends, its part of the output being undefined.
-#include <cuda.h>
-
-#include <cstddef>
-
 #include "paged_kv.cuh"
 
 namespace kvcm {
 namespace {
 
-constexpr int kAttendWarps = 4;                            // consumers
-constexpr int kAttendThreads = (kAttendWarps + 1) * 32;    // and the producer
-constexpr int kTile = 16;                                  // tokens a consumer takes per step
-constexpr int kStep = kTile * kAttendWarps;                // tokens a CTA takes per step
-constexpr int64_t kMinRun = 4;                             // steps of a run: shorter ones are not worth joining
-constexpr int kMaxWorkers = 1024;
+constexpr int kAttendWarps = 4;
+constexpr int kAttendThreads = kAttendWarps * 32;
+constexpr int kTile = 16;                                  // tokens of a tile
+constexpr int64_t kMinRun = 1;                             // steps of a run
+constexpr int kMaxWorkers = 512;
 constexpr int kMaxAttendHeadDim = 256;
 constexpr int kJoinThreads = 256;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -61,17 +54,20 @@ struct AttendParams {
     // workspace
     int64_t *steps_before;  // [batch + 1] steps of all sequences before this one, one KV head and row tile counted
     int4 *runs;             // [workers] where each run begins: sequence, unit, step within the unit (0: nothing is cut)
-    float *part_o;          // [workers * 2][rows][dim]
-    float2 *part_ml;        // [workers * 2][rows] maximum and sum of a share, the maximum in units of log2
+    float *part_o;          // [workers * 2][step_heads][rows][dim]
+    float2 *part_ml;        // [workers * 2][step_heads][rows] maximum and sum of a share, the maximum in units of log2
     float2 *whole_ml;       // [batch][n_q_heads], heads that one CTA finished
     float *scores;          // [batch][n_q_heads][score_stride], in units of log2; null without weights
     int64_t score_stride;
     int32_t batch, n_q_heads, group;
-    int32_t row_tiles;  // tiles of kRows query heads per KV head
-    int32_t units;      // KV heads * row tiles
+    int32_t row_tiles;   // tiles of kRows query heads per KV head
+    int32_t step_heads;  // KV heads of a step, 1, 2 or 4: its four tiles are step_heads heads by step_tokens tokens
+    int32_t step_tokens;
+    int32_t units;       // KV heads / step_heads * row tiles
     int32_t table_tokens;
     int32_t window;
-    int32_t box;  // tokens of a TMA box: the largest power of two up to 16 that divides page_tokens
+    int32_t whole_tiles;  // page_tokens is a multiple of kTile: a tile lies in one page
+    int32_t page_shift;   // log2 of page_tokens, or -1
     float scale_log2;
     int32_t workers;
 };
@@ -87,7 +83,7 @@ __device__ __forceinline__ Span SpanOf(const AttendParams &p, int32_t b) {
     s.len = max(0, min(__ldg(p.lens + b), p.table_tokens));
     s.first = p.window > 0 ? max(0, s.len - p.window) : 0;
     s.base = s.first & ~(kTile - 1);
-    s.steps = (s.len - s.base + kStep - 1) / kStep;
+    s.steps = (s.len - s.base + p.step_tokens - 1) / p.step_tokens;
     return s;
 }
 
@@ -102,12 +98,14 @@ __device__ __forceinline__ float Exp2(float x) {  // results below 2^-126 are ze
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void LoadBox(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t head, int32_t token,
-                                        int32_t page, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
-        "l"(map), "r"(x), "r"(head), "r"(token), "r"(page), "r"(bar)
-        : "memory");
+// 16 bytes, of which the first `bytes` come from src and the rest are zeros.
+__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void CopyWait() {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kPending) : "memory");
 }
 __device__ __forceinline__ void LoadMatrix(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
@@ -151,88 +149,52 @@ __device__ __forceinline__ void SplitPair(float p0, float p1, uint32_t &hi, uint
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// Shapes of the main kernel: kDim (64, 128, 256) is head_dim rounded up, kRows (8, 16) the query heads of a row tile.
-// Two CTAs per SM where the ring and the joined sums leave room, with as many stages as then fit.
-template <int kDim, int kRows>
+// Shapes of the main kernel: kDim (64, 128, 256) is head_dim rounded up.
+template <int kDim>
 struct AttendShape {
-    static constexpr int kHalves = kDim / 64;              // boxes across a row
-    static constexpr int kTileBytes = kTile * kDim * 2;    // of K, and again of V
+    static constexpr int kRowBytes = kDim * 2;
+    static constexpr int kTileBytes = kTile * kRowBytes;  // of K, and again of V
     static constexpr int kStageBytes = kAttendWarps * 2 * kTileBytes;
-    static constexpr int kStages = kDim == 64 ? 5 : (kRows == 16 ? 2 : 3);
+    static constexpr int kStages = kDim == 64 ? 4 : 3;
     static constexpr int kRingBytes = kStages * kStageBytes;
-    static constexpr int kCtasPerSm = kDim == 256 ? 1 : 2;
+    static constexpr int kCtasPerSm = kDim == 256 ? 1 : (kDim == 64 ? 3 : 2);
 };
-
-// What the producer tells the consumers about a step.
-struct __align__(16) StepNote {
-    int32_t b, head0, rows;  // sequence, first query head and number of query heads
-    int32_t step;            // within the unit
-    int32_t next_b, next_head0, next_rows;  // of the share that follows; set in a share's last step
-    uint32_t flags;
-    uint32_t valid[kAttendWarps];  // which of a consumer's 16 tokens take part
-};
-// Shared memory of the main kernel.  The ring comes first: swizzled tiles have to begin on a 1 KB boundary.
-template <int kDim, int kRows>
-struct __align__(1024) AttendShared {
-    using Shape = AttendShape<kDim, kRows>;
-    uint8_t ring[Shape::kRingBytes];
-    float sums[kAttendWarps][kRows][kDim];
-    float2 ml[kAttendWarps][kRows];
-    StepNote notes[Shape::kStages];
-    uint64_t full[Shape::kStages], empty[Shape::kStages], joined;
-    int64_t scan_warp[kAttendWarps + 1];
-    int64_t found_before;
-    int32_t found_b;
-    volatile uint32_t gave_up;
-};
-// What a launch asks for: the structure without its padding to a multiple of 1 KB.
-template <int kDim, int kRows>
-constexpr int AttendSmemBytes() {
-    using Shared = AttendShared<kDim, kRows>;
-    return static_cast<int>(offsetof(Shared, gave_up)) + 4;
-}
-constexpr uint32_t kShareEnds = 1, kShareWhole = 2, kShareBeginsRun = 4, kMoreFollow = 8;
 
 template <typename T, int kDim, int kRows, bool kScores>
-__global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCtasPerSm)
-    AttendPagesKernel(const AttendParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-    using Shape = AttendShape<kDim, kRows>;
+__global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
+    AttendPagesKernel(const __grid_constant__ AttendParams p) {
+    using Shape = AttendShape<kDim>;
     constexpr int kStages = Shape::kStages;
-    extern __shared__ __align__(1024) uint8_t smem[];
-    AttendShared<kDim, kRows> &sh = *reinterpret_cast<AttendShared<kDim, kRows> *>(smem);
+    constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
+    constexpr int kCopyRows = 32 / kPieces;        // rows one copy instruction of a warp covers
+    constexpr int kCopies = kTile / kCopyRows;     // copy instructions per tile of K
+    extern __shared__ __align__(128) uint8_t ring_bytes[];
+    __shared__ float2 join_ml[kAttendWarps][kRows];
+    __shared__ uint32_t valid_masks[kAttendWarps][kStages];
+    __shared__ int64_t scan_warp[kAttendWarps];
+    __shared__ int64_t found_before;
+    __shared__ int32_t found_b;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t ring = SmemAddr(sh.ring);
+    const uint32_t ring = SmemAddr(ring_bytes);
 
     // ---- the run of this CTA: steps [begin, begin + n_steps) of all, found by a scan over the sequences
     const int32_t chunk = (p.batch + kAttendThreads - 1) / kAttendThreads;
     const int32_t b_first = min(p.batch, static_cast<int32_t>(tid) * chunk), b_last = min(p.batch, b_first + chunk);
     int64_t mine = 0;
     for (int32_t b = b_first; b < b_last; ++b) mine += SpanOf(p, b).steps;
-    if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            MbarInit(SmemAddr(&sh.full[s]), 1);
-            MbarInit(SmemAddr(&sh.empty[s]), kAttendWarps);
-        }
-        MbarInit(SmemAddr(&sh.joined), kAttendWarps);
-        sh.gave_up = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        asm volatile("fence.proxy.async;\n" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&k_map) : "memory");
-        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&v_map) : "memory");
-    }
     int64_t inclusive = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const int64_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
         if (lane >= d) inclusive += up;
     }
-    if (lane == 31) sh.scan_warp[warp] = inclusive;
+    if (lane == 31) scan_warp[warp] = inclusive;
     __syncthreads();
     int64_t before = inclusive - mine, all = 0;
 #pragma unroll
-    for (int w = 0; w <= kAttendWarps; ++w) {
-        if (w < static_cast<int>(warp)) before += sh.scan_warp[w];
-        all += sh.scan_warp[w];
+    for (int w = 0; w < kAttendWarps; ++w) {
+        if (w < static_cast<int>(warp)) before += scan_warp[w];
+        all += scan_warp[w];
     }
     const int64_t total = all * p.units;
     const int64_t per = StepsPerRun(total, p.workers);
@@ -268,147 +230,121 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
             if (begin < (at + steps) * p.units) break;
             at += steps;
         }
-        sh.found_b = b;
-        sh.found_before = at * p.units;
+        found_b = b;
+        found_before = at * p.units;
     }
     __syncthreads();
     const int32_t n_steps = static_cast<int32_t>(min(per, total - begin));
-    int32_t b = sh.found_b;
+    int32_t b = found_b;
     Span span = SpanOf(p, b);
-    const int64_t inside = begin - sh.found_before;
+    const int64_t inside = begin - found_before;
     int32_t unit = static_cast<int32_t>(inside / span.steps);
     int32_t step = static_cast<int32_t>(inside - static_cast<int64_t>(unit) * span.steps);
 
-    // Bounded wait; when it runs out, this CTA's other waits end at their first poll.
-    auto wait = [&](uint64_t &bar, uint32_t parity) {
-        if (MbarTryWait(SmemAddr(&bar), parity)) return;
-        if (!BoundedWait(SmemAddr(&bar), parity, sh.gave_up ? 1u : kSpinLimit) && sh.gave_up == 0) {
-            sh.gave_up = 1;
-            if (p.status != nullptr) p.status[2] = 1;
+    if (tid == 0) p.runs[blockIdx.x] = make_int4(b, unit, step, 0);
+
+    const int32_t token_tiles = p.step_tokens / kTile;  // of a step: 4, 2, 1
+    const int32_t my_head = static_cast<int32_t>(warp) / token_tiles;
+    const int32_t my_t = (static_cast<int32_t>(warp) - my_head * token_tiles) * kTile;  // from the step's first token
+    const int32_t kv_groups = p.pools.n_kv_heads / p.step_heads;
+
+    // A place in the run.
+    struct Place {
+        int32_t b, kvg, row_tile, step;
+        Span span;
+        __device__ __forceinline__ void Next(const AttendParams &p, int32_t kv_groups) {  // a step has to follow
+            if (++step < span.steps) return;
+            step = 0;
+            if (++row_tile < p.row_tiles) return;
+            row_tile = 0;
+            if (++kvg < kv_groups) return;
+            kvg = 0;
+            do {
+                span = SpanOf(p, ++b);
+            } while (span.steps == 0);
+        }
+    };
+    Place now;
+    now.b = b;
+    now.kvg = unit / p.row_tiles;
+    now.row_tile = unit - now.kvg * p.row_tiles;
+    now.step = step;
+    now.span = span;
+    Place ask = now;  // of the next tile to load
+
+    // The table entry of the next tile to load: of the whole tile, or of token lane % 16 where tiles cross pages.
+    int32_t ask_page = 0, ask_token = 0;
+    auto look_up = [&]() {
+        const int32_t t0 = ask.span.base + ask.step * p.step_tokens + my_t;
+        const int32_t t = p.whole_tiles ? t0 : t0 + static_cast<int32_t>(lane & (kTile - 1));
+        ask_page = -1;
+        if (t < ask.span.len && (p.whole_tiles ? t + kTile : t + 1) > ask.span.first) {
+            const int32_t page_i = p.page_shift >= 0 ? t >> p.page_shift : t / p.pools.page_tokens;
+            ask_token = t - page_i * p.pools.page_tokens;
+            ask_page = __ldg(p.table + ask.b * p.table_stride + page_i);
+            // a page outside the pool is counted once
+            if ((ask_page < 0 || ask_page >= p.pools.pool_pages) && ask.kvg == 0 && ask.row_tile == 0 && my_head == 0 &&
+                (p.whole_tiles ? lane == 0 : lane < kTile) && (ask_token == 0 || t <= ask.span.first)) {
+                CountSkipped(p.status, static_cast<uint32_t>(ask.b), 1u);
+            }
         }
     };
 
-    if (warp == kAttendWarps) {
-        // ---- producer: one lane per box of `box` tokens
-        if (lane == 0) p.runs[blockIdx.x] = make_int4(b, unit, step, 0);
-        const int32_t boxes = kStep / p.box;  // 4 .. 64
-        const uint32_t box_bits = (1u << p.box) - 1u;
-        int32_t kv = unit / p.row_tiles;
-        int32_t row_tile = unit - kv * p.row_tiles;
-        int32_t share_first = step;
-        int stage = 0;
-        uint32_t parity = 1;  // the first pass over the ring finds every stage sh.empty
-        for (int32_t s = 0; s < n_steps; ++s) {
-            uint32_t valid[2];
-            int32_t page[2], token[2];
-            uint32_t issued = 0;
-            const int32_t t_step = span.base + step * kStep;
-            // table first: its latency passes while the stage is still in use
+    const uint32_t tiles_at = ring + warp * 2 * Shape::kTileBytes;
+    const uint32_t copy_piece = lane % kPieces, copy_row = lane / kPieces;
+    const uint32_t copy_bytes = copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? 16u : 0u;
+    const uint32_t copy_to = copy_row * Shape::kRowBytes + ((copy_piece ^ copy_row) * 16);  // of the first copy
+    const int64_t copy_from = static_cast<int64_t>(copy_row) * p.pools.token_stride + (copy_bytes != 0 ? copy_piece * 16 : 0);
+    const int64_t copy_stride = kCopyRows * p.pools.token_stride;
+    const int64_t v_minus_k = p.pools.v - p.pools.k;
+    // Starts the copies of this warp's tile of the next step; rows that take no part become zeros, so that whatever lies
+    // there cannot reach a product.
+    auto load_tile = [&](int to_stage) {
+        const int32_t t0 = ask.span.base + ask.step * p.step_tokens + my_t;
+        const int32_t begins = max(ask.span.first - t0, 0), ends = min(ask.span.len - t0, kTile);
+        uint32_t valid = ends > begins ? ((1u << ends) - 1u) & ~((1u << begins) - 1u) : 0u;
+        const bool page_ok = ask_page >= 0 && ask_page < p.pools.pool_pages;
+        const int64_t head_off = static_cast<int64_t>(ask.kvg * p.step_heads + my_head) * p.pools.head_stride;
+        const uint32_t to = tiles_at + to_stage * Shape::kStageBytes + copy_to;
+        if (p.whole_tiles) {
+            if (!page_ok) valid = 0;
+            if (valid != 0) {
+                const uint8_t *from = p.pools.k + ask_page * p.pools.page_stride + ask_token * p.pools.token_stride + head_off + copy_from;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int32_t i = r * 32 + static_cast<int32_t>(lane);
-                const int32_t t = t_step + i * p.box;
-                valid[r] = 0;
-                page[r] = -1;
-                token[r] = 0;
-                if (i < boxes && t < span.len && t + p.box > span.first) {
-                    const int32_t page_i = t / p.pools.page_tokens;
-                    token[r] = t - page_i * p.pools.page_tokens;
-                    const int32_t at = __ldg(p.table + b * p.table_stride + page_i);
-                    if (at >= 0 && at < p.pools.pool_pages) {
-                        page[r] = at;
-                        valid[r] = box_bits;
-                        if (t < span.first) valid[r] &= box_bits << (span.first - t);
-                        if (t + p.box > span.len) valid[r] &= box_bits >> (t + p.box - span.len);
-                        ++issued;
-                    } else if (unit == 0 && (token[r] == 0 || t <= span.first)) {
-                        CountSkipped(p.status, static_cast<uint32_t>(b), 1u);  // once for each page
-                    }
+                for (int i = 0; i < kCopies; ++i) {
+                    const uint32_t row = i * kCopyRows + copy_row;
+                    const uint32_t bytes = (valid >> row) & 1u ? copy_bytes : 0u;
+                    const uint32_t at = (to ^ (((i * kCopyRows) & 7) * 16)) + i * kCopyRows * Shape::kRowBytes;
+                    CopyAsync16(at, from, bytes);
+                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes);
+                    from += copy_stride;
                 }
             }
-            const uint32_t all_issued = __reduce_add_sync(0xffffffffu, issued);
-            // a tile's mask, from the boxes that lie in it
-            const int32_t per_tile = kTile / p.box;
+        } else {
+            valid &= __ballot_sync(0xffffffffu, page_ok);
+            const int64_t off = ask_page * p.pools.page_stride + ask_token * p.pools.token_stride + head_off;
+            if (valid != 0) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                uint32_t bits = valid[r] << (((r * 32 + lane) * p.box) & (kTile - 1));
-                for (int d = 1; d < per_tile; d *= 2) bits |= __shfl_xor_sync(0xffffffffu, bits, d);
-                valid[r] = bits;
-            }
-            wait(sh.empty[stage], parity);
-            StepNote &note = sh.notes[stage];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int32_t i = r * 32 + static_cast<int32_t>(lane);
-                if (i < boxes && i % per_tile == 0) note.valid[i / per_tile] = valid[r];
-            }
-            const bool unit_ends = step + 1 == span.steps;
-            const bool share_ends = unit_ends || s + 1 == n_steps;
-            const int32_t this_b = b, this_step = step, this_kv = kv, this_tile = row_tile;
-            uint32_t flags = 0;
-            if (share_ends) {
-                flags = kShareEnds | (share_first == 0 && unit_ends ? kShareWhole : 0u) |
-                        (s == this_step - share_first ? kShareBeginsRun : 0u) | (s + 1 < n_steps ? kMoreFollow : 0u);
-            }
-            ++step;
-            if (share_ends && s + 1 < n_steps) {  // on to the next unit, or the next sequence that has tokens
-                step = share_first = 0;
-                if (++row_tile == p.row_tiles) {
-                    row_tile = 0;
-                    ++kv;
+                for (int i = 0; i < kCopies; ++i) {
+                    const uint32_t row = i * kCopyRows + copy_row;
+                    const int64_t row_off = __shfl_sync(0xffffffffu, off, row);
+                    const uint32_t bytes = (valid >> row) & 1u ? copy_bytes : 0u;
+                    const uint8_t *from = p.pools.k + (bytes != 0 ? row_off + copy_piece * 16 : 0);
+                    const uint32_t at = (to ^ (((i * kCopyRows) & 7) * 16)) + i * kCopyRows * Shape::kRowBytes;
+                    CopyAsync16(at, from, bytes);
+                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes);
                 }
-                if (++unit == p.units) {
-                    unit = kv = 0;
-                    do {
-                        span = SpanOf(p, ++b);
-                    } while (span.steps == 0);
-                }
-            }
-            if (lane == 0) {
-                note.b = this_b;
-                note.head0 = this_kv * p.group + this_tile * kRows;
-                note.rows = min(kRows, p.group - this_tile * kRows);
-                note.step = this_step;
-                note.next_b = b;
-                note.next_head0 = kv * p.group + row_tile * kRows;
-                note.next_rows = min(kRows, p.group - row_tile * kRows);
-                note.flags = flags;
-            }
-            __syncwarp();
-            const uint32_t bar = SmemAddr(&sh.full[stage]);
-            if (lane == 0) MbarArriveExpectTx(bar, all_issued * p.box * kDim * 2 * 2);
-            __syncwarp();
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                if (page[r] >= 0) {
-                    const uint32_t row = (r * 32 + lane) * p.box;  // within the step
-                    const uint32_t to = ring + stage * Shape::kStageBytes + (row / kTile) * 2 * Shape::kTileBytes + (row % kTile) * 128;
-#pragma unroll
-                    for (int h = 0; h < Shape::kHalves; ++h) {
-                        LoadBox(to + h * kTile * 128, &k_map, h * 64, this_kv, token[r], page[r], bar);
-                        LoadBox(to + Shape::kTileBytes + h * kTile * 128, &v_map, h * 64, this_kv, token[r], page[r], bar);
-                    }
-                }
-            }
-            if (++stage == kStages) {
-                stage = 0;
-                parity ^= 1;
             }
         }
-        // nothing may arrive in shared memory that is no longer this CTA's
-        for (int s = 0; s < kStages; ++s) {
-            if (s < n_steps) wait(sh.full[s], ((n_steps - 1 - s) / kStages) & 1);
-        }
-        return;
-    }
+        if (lane == 0) valid_masks[warp][to_stage] = valid;
+    };
 
-    // ---- consumers
     constexpr int kOut = kDim / 8;
     float o[kOut][4];
     uint32_t qa[kDim / 16][kRows == 8 ? 2 : 4];
     float top[2], sum[2];  // of rows lane / 4 and lane / 4 + 8
     auto load_queries = [&](int32_t of_b, int32_t head0, int32_t rows) {
-        const T *q = reinterpret_cast<const T *>(p.query) + of_b * p.q_batch + head0 * p.q_head;
+        const T *q = reinterpret_cast<const T *>(p.query) + of_b * p.q_batch + (head0 + my_head * p.group) * p.q_head;
 #pragma unroll
         for (int ks = 0; ks < kDim / 16; ++ks) {
 #pragma unroll
@@ -430,34 +366,52 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
         top[0] = top[1] = -INFINITY;
         sum[0] = sum[1] = 0.0f;
     };
-    {
-        const int32_t kv = unit / p.row_tiles, row_tile = unit - kv * p.row_tiles;
-        load_queries(b, kv * p.group + row_tile * kRows, min(kRows, p.group - row_tile * kRows));
-        clear();
+
+    look_up();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+        if (s < n_steps) {
+            load_tile(s);
+            if (s + 1 < n_steps) {
+                ask.Next(p, kv_groups);
+                look_up();
+            }
+        }
+        CopyCommit();
     }
+    int32_t head0 = now.kvg * p.step_heads * p.group + now.row_tile * kRows;  // the step's first query head
+    int32_t rows = min(kRows, p.group - now.row_tile * kRows);                // and those of a row tile
+    int32_t share_first = now.step;
+    load_queries(now.b, head0, rows);
+    clear();
+
     // lane's row and 16-byte column in the swizzled tiles, for the K and the V product
     const uint32_t k_row = (lane & 7) + ((lane >> 4) << 3), v_row = lane & 15;
-    const uint32_t k_lane = k_row * 128 + ((((lane >> 3) & 1) ^ (k_row & 7)) * 16);
-    const uint32_t v_lane = Shape::kTileBytes + v_row * 128 + (((lane >> 4) ^ (v_row & 7)) * 16);
+    const uint32_t k_lane = k_row * Shape::kRowBytes + ((((lane >> 3) & 1) ^ (k_row & 7)) * 16);
+    const uint32_t v_lane = Shape::kTileBytes + v_row * Shape::kRowBytes + (((lane >> 4) ^ (v_row & 7)) * 16);
     const int32_t k_steps = (p.pools.head_dim + 15) / 16;  // 16-element pieces of a row that are not padding
     int stage = 0;
-    uint32_t parity = 0, join_parity = 0;
     for (int32_t s = 0; s < n_steps; ++s) {
-        wait(sh.full[stage], parity);
-        const StepNote &note = sh.notes[stage];
-        const uint32_t valid = note.valid[warp];
-        const uint32_t flags = note.flags;
-        const uint32_t tile = ring + stage * Shape::kStageBytes + warp * 2 * Shape::kTileBytes;
+        CopyWait<kStages - 2>();
+        __syncwarp();
+        if (s + kStages - 1 < n_steps) {
+            load_tile(stage == 0 ? kStages - 1 : stage - 1);
+            if (s + kStages < n_steps) {
+                ask.Next(p, kv_groups);
+                look_up();
+            }
+        }
+        CopyCommit();
+        const uint32_t valid = valid_masks[warp][stage];
+        const uint32_t tile = tiles_at + stage * Shape::kStageBytes;
         int64_t score_at = 0;  // where this thread's scores of row lane / 4 go: two pairs of tokens, eight apart
-        int32_t score_rows = 0;
         if (kScores) {
-            score_rows = note.rows;
-            score_at = (static_cast<int64_t>(note.b) * p.n_q_heads + note.head0 + (lane >> 2)) * p.score_stride +
-                       static_cast<int64_t>(note.step) * kStep + warp * kTile + (lane & 3) * 2;
+            score_at = (static_cast<int64_t>(now.b) * p.n_q_heads + head0 + my_head * p.group + (lane >> 2)) * p.score_stride +
+                       static_cast<int64_t>(now.step) * p.step_tokens + my_t + (lane & 3) * 2;
             if (valid == 0) {
 #pragma unroll
                 for (int r = 0; r < kRows / 8; ++r) {
-                    if (static_cast<int>(lane >> 2) + r * 8 < score_rows) {
+                    if (static_cast<int>(lane >> 2) + r * 8 < rows) {
                         float *to = p.scores + score_at + r * 8 * p.score_stride;
                         *reinterpret_cast<float2 *>(to) = make_float2(-INFINITY, -INFINITY);
                         *reinterpret_cast<float2 *>(to + 8) = make_float2(-INFINITY, -INFINITY);
@@ -466,34 +420,39 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
             }
         }
         if (valid != 0) {
-            if (valid != 0xffffu) {
-                // V rows that take no part become zeros: a probability of zero would not undo a NaN there
-                for (uint32_t row = 0; row < kTile; ++row) {
-                    if ((valid >> row) & 1u) continue;
-                    for (uint32_t c = lane; c < kDim / 8; c += 32) {
-                        const uint32_t at = tile + Shape::kTileBytes + (c >> 3) * (kTile * 128) + row * 128 + (c & 7) * 16;
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(at), "r"(0) : "memory");
-                    }
-                }
-                asm volatile("fence.proxy.async;\n" ::: "memory");  // before the stage's next load
-                __syncwarp();
-            }
-            // ---- scores of 16 tokens: two 16x8 products over the head dimension
+            // ---- scores of 16 tokens: two 16x8 products over the head dimension, operands fetched ahead in groups
+            constexpr int kAhead = kDim == 256 ? 4 : 8;
             float c[2][2][4] = {};
 #pragma unroll
-            for (int ks = 0; ks < kDim / 16; ++ks) {
-                if (kDim == 64 || ks < kDim / 32 || ks < k_steps) {
-                    uint32_t kb[4];
-                    LoadMatrix(kb, ((tile + k_lane) ^ ((ks & 3) * 32)) + (ks >> 2) * (kTile * 128));
-                    if constexpr (kRows == 8) {
-                        MatrixMultiply<T>(c[ks & 1][0], qa[ks][0], 0u, qa[ks][1], 0u, kb[0], kb[1]);
-                        MatrixMultiply<T>(c[ks & 1][1], qa[ks][0], 0u, qa[ks][1], 0u, kb[2], kb[3]);
-                    } else {
-                        MatrixMultiply<T>(c[ks & 1][0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[0], kb[1]);
-                        MatrixMultiply<T>(c[ks & 1][1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[2], kb[3]);
+            for (int k0 = 0; k0 < kDim / 16; k0 += kAhead) {
+                uint32_t kb[kAhead][4];
+#pragma unroll
+                for (int i = 0; i < kAhead && k0 + i < kDim / 16; ++i) {
+                    const int ks = k0 + i;
+                    LoadMatrix(kb[i], ((tile + k_lane) ^ ((ks & 3) * 32)) + (ks >> 2) * 128);
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead && k0 + i < kDim / 16; ++i) {
+                    const int ks = k0 + i;
+                    if (kDim == 64 || ks < kDim / 32 || ks < k_steps) {
+                        if constexpr (kRows == 8) {
+                            MatrixMultiply<T>(c[ks & 1][0], qa[ks][0], 0u, qa[ks][1], 0u, kb[i][0], kb[i][1]);
+                            MatrixMultiply<T>(c[ks & 1][1], qa[ks][0], 0u, qa[ks][1], 0u, kb[i][2], kb[i][3]);
+                        } else {
+                            MatrixMultiply<T>(c[ks & 1][0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[i][0], kb[i][1]);
+                            MatrixMultiply<T>(c[ks & 1][1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[i][2], kb[i][3]);
+                        }
                     }
                 }
             }
+            // the first of V's operands, on their way during the softmax
+            constexpr int kVAhead = kDim == 256 ? 2 : kDim / 16;
+            uint32_t vb[kVAhead][4];
+            auto load_v = [&](int j) {
+                LoadMatrixTransposed(vb[j % kVAhead], ((tile + v_lane) ^ ((j & 3) * 32)) + (j >> 2) * 128);
+            };
+#pragma unroll
+            for (int j = 0; j < kVAhead; ++j) load_v(j);
             float x[2][4];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
@@ -513,7 +472,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
             if (kScores) {
 #pragma unroll
                 for (int r = 0; r < kRows / 8; ++r) {
-                    if (static_cast<int>(lane >> 2) + r * 8 < score_rows) {
+                    if (static_cast<int>(lane >> 2) + r * 8 < rows) {
                         float *to = p.scores + score_at + r * 8 * p.score_stride;
                         *reinterpret_cast<float2 *>(to) = make_float2(x[0][r * 2], x[0][r * 2 + 1]);
                         *reinterpret_cast<float2 *>(to + 8) = make_float2(x[1][r * 2], x[1][r * 2 + 1]);
@@ -560,31 +519,36 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
 #pragma unroll
             for (int j = 0; j < kDim / 16; ++j) {
                 if (kDim == 64 || j < kDim / 32 || j < k_steps) {
-                    uint32_t vb[4];
-                    LoadMatrixTransposed(vb, ((tile + v_lane) ^ ((j & 3) * 32)) + (j >> 2) * (kTile * 128));
-                    MatrixMultiply<T>(o[2 * j], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
-                    MatrixMultiply<T>(o[2 * j + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
+                    const uint32_t(&v)[4] = vb[j % kVAhead];
+                    MatrixMultiply<T>(o[2 * j], pa[0], pa[1], pa[2], pa[3], v[0], v[1]);
+                    MatrixMultiply<T>(o[2 * j + 1], pa[0], pa[1], pa[2], pa[3], v[2], v[3]);
                     if constexpr (kRows == 16) {
-                        MatrixMultiply<T>(o[2 * j], pl[0], pl[1], pl[2], pl[3], vb[0], vb[1]);
-                        MatrixMultiply<T>(o[2 * j + 1], pl[0], pl[1], pl[2], pl[3], vb[2], vb[3]);
+                        MatrixMultiply<T>(o[2 * j], pl[0], pl[1], pl[2], pl[3], v[0], v[1]);
+                        MatrixMultiply<T>(o[2 * j + 1], pl[0], pl[1], pl[2], pl[3], v[2], v[3]);
                     }
                 }
+                if (j + kVAhead < kDim / 16) load_v(j + kVAhead);
             }
         }
 
-        if (flags & kShareEnds) {
-            // ---- the share is complete: the warps' sums are sh.joined in shared memory
-            const int32_t rows = note.rows, head0 = note.head0, of_b = note.b;
-            const int32_t next_b = note.next_b, next_head0 = note.next_head0, next_rows = note.next_rows;
-            __syncwarp();
-            if (lane == 0) MbarArrive(SmemAddr(&sh.empty[stage]));
+        __syncwarp();  // the stage may be filled again
+
+        const bool unit_ends = now.step + 1 == now.span.steps;
+        const bool more = s + 1 < n_steps;
+        if (unit_ends || !more) {
+            // ---- the share is complete: the sums of the warps with the same KV head are joined, in the tiles that this
+            // step has used up
+            const bool whole = share_first == 0 && unit_ends;
+            const bool begins_run = s == now.step - share_first;
+            const int32_t of_b = now.b, of_head0 = head0, of_rows = rows;
 #pragma unroll
             for (int r = 0; r < kRows / 8; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                if ((lane & 3) == 0) sh.ml[warp][(lane >> 2) + r * 8] = make_float2(top[r], sum[r]);
+                if ((lane & 3) == 0) join_ml[warp][(lane >> 2) + r * 8] = make_float2(top[r], sum[r]);
             }
-            float *mine_o = &sh.sums[warp][lane >> 2][(lane & 3) * 2];
+            uint8_t *sums = ring_bytes + stage * Shape::kStageBytes;  // warp w's at w * 2 * kTileBytes, [kRows][kDim]
+            float *mine_o = reinterpret_cast<float *>(sums + warp * 2 * Shape::kTileBytes) + (lane >> 2) * kDim + (lane & 3) * 2;
 #pragma unroll
             for (int j = 0; j < kOut; ++j) {
                 if constexpr (kRows == 8) {
@@ -594,33 +558,36 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                     *reinterpret_cast<float2 *>(mine_o + 8 * kDim + j * 8) = make_float2(o[j][2], o[j][3]);
                 }
             }
-            if (flags & kMoreFollow) load_queries(next_b, next_head0, next_rows);  // on its way while the sums are sh.joined
-            __syncwarp();
-            if (lane == 0) MbarArrive(SmemAddr(&sh.joined));
-            wait(sh.joined, join_parity);
-            join_parity ^= 1;
-            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + ((flags & kShareBeginsRun) ? 0 : 1)) * kRows;
-            for (uint32_t i = tid; i < static_cast<uint32_t>(rows) * (kDim / 2); i += kAttendWarps * 32) {
-                const uint32_t row = i / (kDim / 2);
-                const uint32_t d = (i - row * (kDim / 2)) * 2;
+            if (more) {  // the next share's queries are on their way while this one's sums are joined
+                now.Next(p, kv_groups);
+                share_first = 0;
+                head0 = now.kvg * p.step_heads * p.group + now.row_tile * kRows;
+                rows = min(kRows, p.group - now.row_tile * kRows);
+                load_queries(now.b, head0, rows);
+            }
+            __syncthreads();
+            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (begins_run ? 0 : 1)) * p.step_heads * kRows;
+            for (int32_t i = tid; i < p.step_heads * of_rows * (kDim / 2); i += kAttendThreads) {
+                const int32_t head_row = i / (kDim / 2), kv_i = head_row / of_rows, row = head_row - kv_i * of_rows;
+                const int32_t d = (i - head_row * (kDim / 2)) * 2;
                 float m = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, sh.ml[w][row].x);
+                for (int32_t w = kv_i * token_tiles; w < (kv_i + 1) * token_tiles; ++w) m = fmaxf(m, join_ml[w][row].x);
+                const float use = m == -INFINITY ? 0.0f : m;
                 float l = 0.0f;
                 float2 acc = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < kAttendWarps; ++w) {
-                    const float2 ml = sh.ml[w][row];
-                    const float f = Exp2(ml.x - (m == -INFINITY ? 0.0f : m));
-                    const float2 part = *reinterpret_cast<const float2 *>(&sh.sums[w][row][d]);
+                for (int32_t w = kv_i * token_tiles; w < (kv_i + 1) * token_tiles; ++w) {
+                    const float2 ml = join_ml[w][row];
+                    const float f = Exp2(ml.x - use);
+                    const float2 part = *reinterpret_cast<const float2 *>(
+                        reinterpret_cast<const float *>(sums + w * 2 * Shape::kTileBytes) + row * kDim + d);
                     l += ml.y * f;
                     acc.x += part.x * f;
                     acc.y += part.y * f;
                 }
-                if (flags & kShareWhole) {
+                if (whole) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const int64_t head_at = static_cast<int64_t>(of_b) * p.n_q_heads + head0 + row;
-                    if (d < static_cast<uint32_t>(p.pools.head_dim)) {
+                    const int64_t head_at = static_cast<int64_t>(of_b) * p.n_q_heads + of_head0 + kv_i * p.group + row;
+                    if (d < p.pools.head_dim) {
                         T *to = reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim + d;
                         *reinterpret_cast<typename Half16<T>::Pair *>(to) = Half16<T>::FromFloat2(acc.x * inv, acc.y * inv);
                     }
@@ -629,24 +596,19 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kRows>::kCta
                         if (p.lse != nullptr) p.lse[head_at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
                     }
                 } else {
-                    *reinterpret_cast<float2 *>(p.part_o + (slot + row) * kDim + d) = acc;
-                    if (d == 0) p.part_ml[slot + row] = make_float2(m, l);
+                    const int64_t to = slot + kv_i * kRows + row;
+                    *reinterpret_cast<float2 *>(p.part_o + to * kDim + d) = acc;
+                    if (d == 0) p.part_ml[to] = make_float2(m, l);
                 }
             }
-            __syncwarp();
-            if (lane == 0) MbarArrive(SmemAddr(&sh.joined));
-            wait(sh.joined, join_parity);  // the sums may be overwritten
-            join_parity ^= 1;
+            __syncthreads();  // the sums may be overwritten
             clear();
         } else {
-            __syncwarp();
-            if (lane == 0) MbarArrive(SmemAddr(&sh.empty[stage]));
+            now.Next(p, kv_groups);
         }
-        if (++stage == kStages) {
-            stage = 0;
-            parity ^= 1;
-        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
     }
+    CopyWait<0>();
 }
 
 // Where the shares of a unit lie: runs [first, last]; the share of run w is in slot 2 w + (the unit begins within the run).
@@ -691,7 +653,7 @@ struct Partial {
 //
 // Weights: the steps of all sequences and weight heads are cut into equal runs again.
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendParams p, int32_t weight_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 4) JoinSharesKernel(const AttendParams p, int32_t weight_blocks) {
     __shared__ Partial partials[kJoinThreads / 32];
     __shared__ int32_t found_b;
     extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count for a weight head
@@ -706,10 +668,10 @@ __global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendPar
         const int64_t steps = p.steps_before[run.x + 1] - p.steps_before[run.x];
         const Shares sh = SharesAt(w * per - run.z, steps, per);
         const int32_t cuts = sh.last - sh.first, cut = w - sh.first - 1;
-        const int32_t kv = run.y / p.row_tiles, row_tile = run.y - kv * p.row_tiles;
+        const int32_t kvg = run.y / p.row_tiles, row_tile = run.y - kvg * p.row_tiles;
         const int32_t rows = min(kRows, p.group - row_tile * kRows);
-        const int64_t head0 = static_cast<int64_t>(run.x) * p.n_q_heads + kv * p.group + row_tile * kRows;
-        const int32_t fours = rows * (kDim / 4);                   // groups of four output elements
+        const int64_t head0 = static_cast<int64_t>(run.x) * p.n_q_heads + kvg * p.step_heads * p.group + row_tile * kRows;
+        const int32_t fours = p.step_heads * rows * (kDim / 4);    // groups of four output elements
         const int32_t mine = (fours + cuts - 1) / cuts;            // this block's
         int32_t lanes = 1;                                         // thread groups per pass, a power of two
         while (lanes < mine && lanes < kJoinThreads) lanes *= 2;
@@ -718,12 +680,14 @@ __global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendPar
         for (int32_t base = 0; base < mine; base += lanes) {
             const int32_t four = cut * mine + base + at;
             const bool live = base + at < mine && four < fours;
-            const int32_t row = live ? four / (kDim / 4) : 0, d = live ? (four - row * (kDim / 4)) * 4 : 0;
+            const int32_t head_row = live ? four / (kDim / 4) : 0, d = live ? (four - head_row * (kDim / 4)) * 4 : 0;
+            const int32_t kv_i = head_row / rows, row = head_row - kv_i * rows;
+            const int64_t head_at = head0 + kv_i * p.group + row;
             Partial acc = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
             if (live) {
 #pragma unroll 4
                 for (int32_t i = sh.first + part; i <= sh.last; i += parts) {
-                    const int64_t slot = sh.Slot(i) * kRows + row;
+                    const int64_t slot = (sh.Slot(i) * p.step_heads + kv_i) * kRows + row;
                     const float2 ml = __ldcg(p.part_ml + slot);
                     acc.Add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d)));
                 }
@@ -752,11 +716,11 @@ __global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendPar
             if (live && part == 0) {
                 const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
                 if (d < p.pools.head_dim) {  // head_dim is a multiple of eight
-                    auto *to = reinterpret_cast<typename Half16<T>::Pair *>(reinterpret_cast<T *>(p.out) + (head0 + row) * p.pools.head_dim + d);
+                    auto *to = reinterpret_cast<typename Half16<T>::Pair *>(reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim + d);
                     to[0] = Half16<T>::FromFloat2(acc.o.x * inv, acc.o.y * inv);
                     to[1] = Half16<T>::FromFloat2(acc.o.z * inv, acc.o.w * inv);
                 }
-                if (d == 0 && p.lse != nullptr) p.lse[head0 + row] = acc.l == 0.0f ? -INFINITY : acc.m * kLn2 + logf(acc.l);
+                if (d == 0 && p.lse != nullptr) p.lse[head_at] = acc.l == 0.0f ? -INFINITY : acc.m * kLn2 + logf(acc.l);
             }
         }
         return;
@@ -791,7 +755,8 @@ __global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendPar
         for (int32_t i = warp; i < n_heads; i += kJoinThreads / 32) {
             const int32_t head = head0 + i;
             const int32_t kv = head / p.group, in_group = head - kv * p.group;
-            const int64_t unit = static_cast<int64_t>(kv) * p.row_tiles + in_group / kRows;
+            const int32_t kvg = kv / p.step_heads, kv_i = kv - kvg * p.step_heads;
+            const int64_t unit = static_cast<int64_t>(kvg) * p.row_tiles + in_group / kRows;
             const Shares sh = SharesAt(before * p.units + unit * span.steps, span.steps, per);
             float m = -INFINITY, l = 0.0f;
             if (sh.first == sh.last) {
@@ -800,7 +765,7 @@ __global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendPar
                 l = ml.y;
             } else {
                 for (int32_t w = sh.first + lane; w <= sh.last; w += 32) {
-                    const float2 ml = __ldcg(p.part_ml + sh.Slot(w) * kRows + in_group % kRows);
+                    const float2 ml = __ldcg(p.part_ml + (sh.Slot(w) * p.step_heads + kv_i) * kRows + in_group % kRows);
                     const float grown = fmaxf(m, ml.x);
                     const float use = grown == -INFINITY ? 0.0f : grown;
                     l = l * Exp2(m - use) + ml.y * Exp2(ml.x - use);
@@ -822,16 +787,24 @@ __global__ void __launch_bounds__(kJoinThreads) JoinSharesKernel(const AttendPar
         const float *scores = p.scores + (static_cast<int64_t>(b) * p.n_q_heads + head0) * p.score_stride;
         const float *w_in = p.weights + b * p.w_batch + wh * p.w_head;
         float *w_out = p.weights_out + b * p.wo_batch + wh * p.wo_head;
-        const int32_t last = min((step0 + steps) * kStep, span.len - span.base);  // relative to the span's base
-        for (int32_t t = step0 * kStep + static_cast<int32_t>(tid); t < last; t += kJoinThreads) {
-            if (span.base + t < span.first) continue;
-            float received = 0.0f;
-#pragma unroll 4
+        const int32_t last = min((step0 + steps) * p.step_tokens, span.len - span.base);  // relative to the span's base
+        constexpr int kAtOnce = 4;  // tokens of a thread, whose loads are in flight together
+        for (int32_t t0 = step0 * p.step_tokens + static_cast<int32_t>(tid); t0 < last; t0 += kAtOnce * kJoinThreads) {
+            float received[kAtOnce] = {};
+#pragma unroll 2
             for (int32_t i = 0; i < n_heads; ++i) {
                 const float2 ml = head_ml[i];
-                received += Exp2(__ldcg(scores + i * p.score_stride + t) - ml.x) * ml.y;
+                const float *row = scores + i * p.score_stride + t0;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    if (t0 + j * kJoinThreads < last) received[j] += Exp2(__ldcg(row + j * kJoinThreads) - ml.x) * ml.y;
+                }
             }
-            w_out[span.base + t] = w_in[span.base + t] + received;
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int32_t t = span.base + t0 + j * kJoinThreads;
+                if (t0 + j * kJoinThreads < last && t >= span.first) w_out[t] = w_in[t] + received[j];
+            }
         }
         at += steps;
         if (at == (before + span.steps) * p.n_weight_heads) ++b;
@@ -852,65 +825,28 @@ AttendWorkspace LayOut(int32_t batch, int32_t n_q_heads, int32_t group, int32_t 
     w.steps_before = 0;
     w.runs = Aligned((static_cast<int64_t>(batch) + 1) * 8);
     w.part_o = w.runs + Aligned(int64_t{kMaxWorkers} * 16);
-    w.part_ml = w.part_o + Aligned(int64_t{kMaxWorkers} * 2 * rows * dim * 4);
-    w.whole_ml = w.part_ml + Aligned(int64_t{kMaxWorkers} * 2 * rows * 8);
+    w.part_ml = w.part_o + Aligned(int64_t{kMaxWorkers} * 2 * kAttendWarps * rows * dim * 4);
+    w.whole_ml = w.part_ml + Aligned(int64_t{kMaxWorkers} * 2 * kAttendWarps * rows * 8);
     w.scores = w.whole_ml + (with_weights ? Aligned(static_cast<int64_t>(batch) * n_q_heads * 8) : 0);
-    w.score_stride = (table_tokens + kStep - 1) / kStep * kStep + kStep;  // a window may begin within a tile
+    // whole steps from a base that may lie up to 15 tokens before the first
+    w.score_stride = (table_tokens + kTile * kAttendWarps - 1) / (kTile * kAttendWarps) * (kTile * kAttendWarps) + kTile * kAttendWarps;
     w.total = w.scores + (with_weights ? Aligned(static_cast<int64_t>(batch) * n_q_heads * w.score_stride * 4) : 0);
     return w;
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver's encoder of tensor maps, looked up once.
-EncodeTiled GetEncodeTiled() {
-    static const EncodeTiled fn = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            f = nullptr;
-        }
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return fn;
-}
-
-// One pool as a tensor of [page][token][head][element]; a box is `box` tokens of one head by 64 elements, elements
-// behind head_dim read as zeros.
-bool MapPool(const AttendParams &p, uint8_t *pool, bool bf16, CUtensorMap *map) {
-    const EncodeTiled encode = GetEncodeTiled();
-    if (encode == nullptr) return false;
-    // the stride of an axis of length one is not used, but has to be well-formed
-    auto stride = [](int64_t bytes, int64_t length) { return static_cast<cuuint64_t>(length > 1 ? bytes : 16); };
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.pools.head_dim), static_cast<cuuint64_t>(p.pools.n_kv_heads),
-                                static_cast<cuuint64_t>(p.pools.page_tokens), static_cast<cuuint64_t>(p.pools.pool_pages)};
-    const cuuint64_t strides[3] = {stride(p.pools.head_stride, p.pools.n_kv_heads),
-                                   stride(p.pools.token_stride, p.pools.page_tokens),
-                                   stride(p.pools.page_stride, p.pools.pool_pages)};
-    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(p.box), 1};
-    const cuuint32_t steps[4] = {1, 1, 1, 1};
-    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, pool, dims, strides, box,
-                  steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int kDim, int kRows, bool kScores>
-void LaunchAttend(AttendParams p, const CUtensorMap &k_map, const CUtensorMap &v_map, cudaStream_t stream) {
-    using Shape = AttendShape<kDim, kRows>;
-    static_assert((AttendSmemBytes<kDim, kRows>() + 1024) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
+void LaunchAttend(AttendParams p, cudaStream_t stream) {
+    using Shape = AttendShape<kDim>;
+    static_assert((Shape::kRingBytes + 2048) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
     auto *main_kernel = AttendPagesKernel<T, kDim, kRows, kScores>;
     auto *join_kernel = JoinSharesKernel<T, kDim, kRows>;
-    EnsureDynamicSmem(main_kernel, AttendSmemBytes<kDim, kRows>());
+    EnsureDynamicSmem(main_kernel, Shape::kRingBytes);
     const int32_t sm_count = GetDeviceInfo().sm_count;
     p.workers = std::min(kMaxWorkers, sm_count * Shape::kCtasPerSm);
-    main_kernel<<<p.workers, kAttendThreads, AttendSmemBytes<kDim, kRows>(), stream>>>(p, k_map, v_map);
+    main_kernel<<<p.workers, kAttendThreads, Shape::kRingBytes, stream>>>(p);
 
     // The second kernel's blocks wait on the device for the first kernel's end, their launch overlaps it.
-    const int32_t weight_blocks = kScores ? 2 * sm_count : 0;
+    const int32_t weight_blocks = kScores ? 8 * sm_count : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.workers + weight_blocks);
     cfg.blockDim = dim3(kJoinThreads);
@@ -925,22 +861,22 @@ void LaunchAttend(AttendParams p, const CUtensorMap &k_map, const CUtensorMap &v
 }
 
 template <typename T, int kDim>
-void DispatchAttend(const AttendParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t stream) {
+void DispatchAttend(const AttendParams &p, cudaStream_t stream) {
     if (p.group <= 8) {
-        p.scores != nullptr ? LaunchAttend<T, kDim, 8, true>(p, k, v, stream) : LaunchAttend<T, kDim, 8, false>(p, k, v, stream);
+        p.scores != nullptr ? LaunchAttend<T, kDim, 8, true>(p, stream) : LaunchAttend<T, kDim, 8, false>(p, stream);
     } else {
-        p.scores != nullptr ? LaunchAttend<T, kDim, 16, true>(p, k, v, stream) : LaunchAttend<T, kDim, 16, false>(p, k, v, stream);
+        p.scores != nullptr ? LaunchAttend<T, kDim, 16, true>(p, stream) : LaunchAttend<T, kDim, 16, false>(p, stream);
     }
 }
 
 template <typename T>
-void DispatchAttend(const AttendParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t stream) {
+void DispatchAttend(const AttendParams &p, cudaStream_t stream) {
     if (p.pools.head_dim <= 64) {
-        DispatchAttend<T, 64>(p, k, v, stream);
+        DispatchAttend<T, 64>(p, stream);
     } else if (p.pools.head_dim <= 128) {
-        DispatchAttend<T, 128>(p, k, v, stream);
+        DispatchAttend<T, 128>(p, stream);
     } else {
-        DispatchAttend<T, 256>(p, k, v, stream);
+        DispatchAttend<T, 256>(p, stream);
     }
 }
 
@@ -1020,19 +956,21 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.group = group;
     const int rows = group <= 8 ? 8 : 16;
     p.row_tiles = (group + rows - 1) / rows;
-    p.units = pools->n_kv_heads * p.row_tiles;
+    p.step_heads = 1;
+    p.step_tokens = kTile * kAttendWarps / p.step_heads;
+    p.units = pools->n_kv_heads / p.step_heads * p.row_tiles;
     p.table_tokens = static_cast<int32_t>(table_tokens);
     p.window = window;
     p.scale_log2 = scale * kLog2e;
-    p.box = kTile;
-    while (pools->page_tokens % p.box != 0) p.box /= 2;
-    const bool bf16 = pools->dtype == KVCM_DTYPE_BF16;
-    CUtensorMap k_map, v_map;
-    if (!MapPool(p, p.pools.k, bf16, &k_map) || !MapPool(p, p.pools.v, bf16, &v_map)) return KVCM_ER_CUDAMEMCPY_ERROR;
-    if (bf16) {
-        DispatchAttend<__nv_bfloat16>(p, k_map, v_map, AsStream(stream));
+    p.whole_tiles = pools->page_tokens % kTile == 0;
+    p.page_shift = -1;
+    for (int32_t i = 0; i < 31; ++i) {
+        if (pools->page_tokens == 1 << i) p.page_shift = i;
+    }
+    if (pools->dtype == KVCM_DTYPE_BF16) {
+        DispatchAttend<__nv_bfloat16>(p, AsStream(stream));
     } else {
-        DispatchAttend<__half>(p, k_map, v_map, AsStream(stream));
+        DispatchAttend<__half>(p, AsStream(stream));
     }
     return LaunchStatus();
 }
