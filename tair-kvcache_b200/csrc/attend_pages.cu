@@ -33,7 +33,7 @@ constexpr int kTile = 16;                                  // tokens of a tile
 constexpr int64_t kMinRun = 1;                             // steps of a run
 constexpr int kMaxWorkers = 512;
 constexpr int kMaxAttendHeadDim = 256;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -52,8 +52,6 @@ struct AttendParams {
     int64_t w_batch, w_head, wo_batch, wo_head;
     int32_t n_weight_heads;
     // workspace
-    int64_t *steps_before;  // [batch + 1] steps of all sequences before this one, one KV head and row tile counted
-    int4 *runs;             // [workers] where each run begins: sequence, unit, step within the unit (0: nothing is cut)
     float *part_o;          // [workers * 2][step_heads][rows][dim]
     float2 *part_ml;        // [workers * 2][step_heads][rows] maximum and sum of a share, the maximum in units of log2
     float2 *whole_ml;       // [batch][n_q_heads], heads that one CTA finished
@@ -87,15 +85,80 @@ __device__ __forceinline__ Span SpanOf(const AttendParams &p, int32_t b) {
     return s;
 }
 
+// a / b, in 32 bits where they do: a 64-bit division takes several times as long.
+__device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
+    return (a | b) <= 0xffffffffll ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 // Steps per run, the same in both kernels.
 __device__ __forceinline__ int64_t StepsPerRun(int64_t all, int32_t workers) {
-    const int64_t per = (all + workers - 1) / workers;
+    const int64_t per = Divide(all + workers - 1, workers);
     return per > kMinRun ? per : kMinRun;
+}
+
+// The steps of all sequences numbered through, each sequence's `times` over.
+struct StepScan {
+    int64_t mine, before, all;  // of this thread's sequences, of those before them, of the batch; once over
+    int32_t b_first, b_last;
+};
+
+// Every thread of the block takes part; `warp_sums` has a word per warp.
+template <int kThreads>
+__device__ __forceinline__ StepScan ScanSteps(const AttendParams &p, int64_t *warp_sums) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int32_t chunk = (p.batch + kThreads - 1) / kThreads;
+    StepScan s;
+    s.b_first = min(p.batch, static_cast<int32_t>(tid) * chunk);
+    s.b_last = min(p.batch, s.b_first + chunk);
+    s.mine = 0;
+    for (int32_t b = s.b_first; b < s.b_last; ++b) s.mine += SpanOf(p, b).steps;
+    int64_t inclusive = s.mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
+        if (lane >= d) inclusive += up;
+    }
+    if (lane == 31) warp_sums[warp] = inclusive;
+    __syncthreads();
+    s.before = inclusive - s.mine;
+    s.all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < static_cast<int>(warp)) s.before += warp_sums[w];
+        s.all += warp_sums[w];
+    }
+    return s;
+}
+
+struct Place64 {
+    int64_t before;  // steps of the sequences before b, `times` over
+    int32_t b;
+};
+
+// Where step x, which has to exist, lies.  Ends with a barrier.
+__device__ __forceinline__ void FindStep(const AttendParams &p, const StepScan &s, int64_t times, int64_t x, Place64 *found) {
+    if (s.before * times <= x && x < (s.before + s.mine) * times) {
+        int64_t at = s.before;
+        int32_t b = s.b_first;
+        for (;; ++b) {
+            const int32_t steps = SpanOf(p, b).steps;
+            if (x < (at + steps) * times) break;
+            at += steps;
+        }
+        found->b = b;
+        found->before = at * times;
+    }
+    __syncthreads();
 }
 
 __device__ __forceinline__ float Exp2(float x) {  // results below 2^-126 are zero
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float Log2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
 // 16 bytes, of which the first `bytes` come from src and the rest are zeros.
@@ -150,20 +213,24 @@ __device__ __forceinline__ void SplitPair(float p0, float p1, uint32_t &hi, uint
 }
 
 // Shapes of the main kernel: kDim (64, 128, 256) is head_dim rounded up.
-template <int kDim>
+template <int kDim, bool kScores>
 struct AttendShape {
     static constexpr int kRowBytes = kDim * 2;
     static constexpr int kTileBytes = kTile * kRowBytes;  // of K, and again of V
     static constexpr int kStageBytes = kAttendWarps * 2 * kTileBytes;
-    static constexpr int kStages = kDim == 64 ? 4 : 3;
+    // Warps hide one another's latencies better than deeper rings do: three CTAs of two stages against two of three
+    // measured 181 against 185 us on the ragged batch, 138 against 161 with a head_dim of 80 - where registers allow.
+    static constexpr int kCtasPerSm = kDim == 256 ? 1 : (kDim == 64 || !kScores ? 3 : 2);
+    static constexpr int kStages = kDim == 64 ? 4 : (kDim == 128 && !kScores ? 2 : 3);
+    static constexpr int kAhead = kDim == 64 || kCtasPerSm == 2 ? 8 : 4;              // K operands fetched together
+    static constexpr int kVAhead = kDim == 64 ? 4 : (kCtasPerSm == 2 ? kDim / 16 : 2);  // and V operands
     static constexpr int kRingBytes = kStages * kStageBytes;
-    static constexpr int kCtasPerSm = kDim == 256 ? 1 : (kDim == 64 ? 3 : 2);
 };
 
 template <typename T, int kDim, int kRows, bool kScores>
-__global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
+__global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kCtasPerSm)
     AttendPagesKernel(const __grid_constant__ AttendParams p) {
-    using Shape = AttendShape<kDim>;
+    using Shape = AttendShape<kDim, kScores>;
     constexpr int kStages = Shape::kStages;
     constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
     constexpr int kCopyRows = 32 / kPieces;        // rows one copy instruction of a warp covers
@@ -172,41 +239,19 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
     __shared__ float2 join_ml[kAttendWarps][kRows];
     __shared__ uint32_t valid_masks[kAttendWarps][kStages];
     __shared__ int64_t scan_warp[kAttendWarps];
-    __shared__ int64_t found_before;
-    __shared__ int32_t found_b;
+    __shared__ Place64 found;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = SmemAddr(ring_bytes);
 
     // ---- the run of this CTA: steps [begin, begin + n_steps) of all, found by a scan over the sequences
-    const int32_t chunk = (p.batch + kAttendThreads - 1) / kAttendThreads;
-    const int32_t b_first = min(p.batch, static_cast<int32_t>(tid) * chunk), b_last = min(p.batch, b_first + chunk);
-    int64_t mine = 0;
-    for (int32_t b = b_first; b < b_last; ++b) mine += SpanOf(p, b).steps;
-    int64_t inclusive = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
-        if (lane >= d) inclusive += up;
-    }
-    if (lane == 31) scan_warp[warp] = inclusive;
-    __syncthreads();
-    int64_t before = inclusive - mine, all = 0;
-#pragma unroll
-    for (int w = 0; w < kAttendWarps; ++w) {
-        if (w < static_cast<int>(warp)) before += scan_warp[w];
-        all += scan_warp[w];
-    }
-    const int64_t total = all * p.units;
+    const StepScan scan = ScanSteps<kAttendThreads>(p, scan_warp);
+    const int64_t total = scan.all * p.units;
     const int64_t per = StepsPerRun(total, p.workers);
     const int64_t begin = blockIdx.x * per;
-    if (blockIdx.x == 0) {  // the second kernel reads where each sequence begins
-        int64_t at = before;
-        for (int32_t b = b_first; b < b_last; ++b) {
-            p.steps_before[b] = at;
-            at += SpanOf(p, b).steps;
-            if (p.status != nullptr && __ldg(p.lens + b) > p.table_tokens) CountSkipped(p.status, b, 1u);
+    if (blockIdx.x == 0 && p.status != nullptr) {
+        for (int32_t b = scan.b_first; b < scan.b_last; ++b) {
+            if (__ldg(p.lens + b) > p.table_tokens) CountSkipped(p.status, b, 1u);
         }
-        if (tid == 0) p.steps_before[p.batch] = all;
     }
     // Sequences without tokens belong to no run: zeros, here.
     for (int32_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -218,30 +263,14 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
         }
     }
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    if (begin >= total) {
-        if (tid == 0) p.runs[blockIdx.x] = make_int4(0, 0, 0, 0);
-        return;
-    }
-    if (before * p.units <= begin && begin < (before + mine) * p.units) {
-        int64_t at = before;
-        int32_t b = b_first;
-        for (;; ++b) {
-            const int32_t steps = SpanOf(p, b).steps;
-            if (begin < (at + steps) * p.units) break;
-            at += steps;
-        }
-        found_b = b;
-        found_before = at * p.units;
-    }
-    __syncthreads();
+    if (begin >= total) return;
+    FindStep(p, scan, p.units, begin, &found);
     const int32_t n_steps = static_cast<int32_t>(min(per, total - begin));
-    int32_t b = found_b;
-    Span span = SpanOf(p, b);
-    const int64_t inside = begin - found_before;
-    int32_t unit = static_cast<int32_t>(inside / span.steps);
-    int32_t step = static_cast<int32_t>(inside - static_cast<int64_t>(unit) * span.steps);
-
-    if (tid == 0) p.runs[blockIdx.x] = make_int4(b, unit, step, 0);
+    const int32_t b = found.b;
+    const Span span = SpanOf(p, b);
+    const int64_t inside = begin - found.before;
+    const int32_t unit = static_cast<int32_t>(Divide(inside, span.steps));
+    const int32_t step = static_cast<int32_t>(inside - static_cast<int64_t>(unit) * span.steps);
 
     const int32_t token_tiles = p.step_tokens / kTile;  // of a step: 4, 2, 1
     const int32_t my_head = static_cast<int32_t>(warp) / token_tiles;
@@ -282,11 +311,15 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
             const int32_t page_i = p.page_shift >= 0 ? t >> p.page_shift : t / p.pools.page_tokens;
             ask_token = t - page_i * p.pools.page_tokens;
             ask_page = __ldg(p.table + ask.b * p.table_stride + page_i);
-            // a page outside the pool is counted once
-            if ((ask_page < 0 || ask_page >= p.pools.pool_pages) && ask.kvg == 0 && ask.row_tile == 0 && my_head == 0 &&
-                (p.whole_tiles ? lane == 0 : lane < kTile) && (ask_token == 0 || t <= ask.span.first)) {
-                CountSkipped(p.status, static_cast<uint32_t>(ask.b), 1u);
-            }
+        }
+    };
+
+    // A page outside the pool is counted once: at its first token, or at the first that is attended.
+    auto report_page = [&](int32_t t0, int32_t begins) {
+        const int32_t t = p.whole_tiles ? t0 + begins : t0 + static_cast<int32_t>(lane & (kTile - 1));
+        const bool mine = p.whole_tiles ? lane == 0 : lane < kTile && t >= ask.span.first && t < ask.span.len;
+        if (mine && my_head == 0 && ask.kvg == 0 && ask.row_tile == 0 && (ask_token == 0 || t == ask.span.first)) {
+            CountSkipped(p.status, static_cast<uint32_t>(ask.b), 1u);
         }
     };
 
@@ -304,6 +337,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
         const int32_t begins = max(ask.span.first - t0, 0), ends = min(ask.span.len - t0, kTile);
         uint32_t valid = ends > begins ? ((1u << ends) - 1u) & ~((1u << begins) - 1u) : 0u;
         const bool page_ok = ask_page >= 0 && ask_page < p.pools.pool_pages;
+        if (!page_ok && valid != 0) report_page(t0, begins);
         const int64_t head_off = static_cast<int64_t>(ask.kvg * p.step_heads + my_head) * p.pools.head_stride;
         const uint32_t to = tiles_at + to_stage * Shape::kStageBytes + copy_to;
         if (p.whole_tiles) {
@@ -367,41 +401,38 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
         sum[0] = sum[1] = 0.0f;
     };
 
-    look_up();
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        if (s < n_steps) {
-            load_tile(s);
-            if (s + 1 < n_steps) {
-                ask.Next(p, kv_groups);
-                look_up();
-            }
-        }
-        CopyCommit();
-    }
-    int32_t head0 = now.kvg * p.step_heads * p.group + now.row_tile * kRows;  // the step's first query head
-    int32_t rows = min(kRows, p.group - now.row_tile * kRows);                // and those of a row tile
-    int32_t share_first = now.step;
-    load_queries(now.b, head0, rows);
-    clear();
-
     // lane's row and 16-byte column in the swizzled tiles, for the K and the V product
     const uint32_t k_row = (lane & 7) + ((lane >> 4) << 3), v_row = lane & 15;
     const uint32_t k_lane = k_row * Shape::kRowBytes + ((((lane >> 3) & 1) ^ (k_row & 7)) * 16);
     const uint32_t v_lane = Shape::kTileBytes + v_row * Shape::kRowBytes + (((lane >> 4) ^ (v_row & 7)) * 16);
     const int32_t k_steps = (p.pools.head_dim + 15) / 16;  // 16-element pieces of a row that are not padding
-    int stage = 0;
-    for (int32_t s = 0; s < n_steps; ++s) {
+    int32_t head0 = 0, rows = 0, share_first = now.step;
+    bool fresh = true;
+    int stage = 0, to_stage = 0;
+    // Iteration s works on step s, loads step s + kStages - 1 and looks up the one after that; the first kStages iterations
+    // only fill the ring.  (One copy of the code: a run is short, and instructions that are met for the first time come
+    // from L2.)
+    for (int32_t s = -kStages; s < n_steps; ++s) {
+        const int32_t asked = s + kStages - 1;
         CopyWait<kStages - 2>();
         __syncwarp();
-        if (s + kStages - 1 < n_steps) {
-            load_tile(stage == 0 ? kStages - 1 : stage - 1);
-            if (s + kStages < n_steps) {
-                ask.Next(p, kv_groups);
-                look_up();
-            }
+        if (asked >= 0) {
+            if (asked < n_steps) load_tile(to_stage);
+            CopyCommit();
+            to_stage = to_stage + 1 == kStages ? 0 : to_stage + 1;
         }
-        CopyCommit();
+        if (asked + 1 < n_steps) {
+            if (asked >= 0) ask.Next(p, kv_groups);
+            look_up();
+        }
+        if (s < 0) continue;
+        if (fresh) {
+            fresh = false;
+            head0 = now.kvg * p.step_heads * p.group + now.row_tile * kRows;  // the step's first query head
+            rows = min(kRows, p.group - now.row_tile * kRows);                // and those of a row tile
+            load_queries(now.b, head0, rows);
+            clear();
+        }
         const uint32_t valid = valid_masks[warp][stage];
         const uint32_t tile = tiles_at + stage * Shape::kStageBytes;
         int64_t score_at = 0;  // where this thread's scores of row lane / 4 go: two pairs of tokens, eight apart
@@ -421,7 +452,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
         }
         if (valid != 0) {
             // ---- scores of 16 tokens: two 16x8 products over the head dimension, operands fetched ahead in groups
-            constexpr int kAhead = kDim == 256 ? 4 : 8;
+            constexpr int kAhead = Shape::kAhead;
             float c[2][2][4] = {};
 #pragma unroll
             for (int k0 = 0; k0 < kDim / 16; k0 += kAhead) {
@@ -446,7 +477,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
                 }
             }
             // the first of V's operands, on their way during the softmax
-            constexpr int kVAhead = kDim == 256 ? 2 : kDim / 16;
+            constexpr int kVAhead = Shape::kVAhead;
             uint32_t vb[kVAhead][4];
             auto load_v = [&](int j) {
                 LoadMatrixTransposed(vb[j % kVAhead], ((tile + v_lane) ^ ((j & 3) * 32)) + (j >> 2) * 128);
@@ -540,7 +571,6 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
             // step has used up
             const bool whole = share_first == 0 && unit_ends;
             const bool begins_run = s == now.step - share_first;
-            const int32_t of_b = now.b, of_head0 = head0, of_rows = rows;
 #pragma unroll
             for (int r = 0; r < kRows / 8; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
@@ -558,17 +588,10 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
                     *reinterpret_cast<float2 *>(mine_o + 8 * kDim + j * 8) = make_float2(o[j][2], o[j][3]);
                 }
             }
-            if (more) {  // the next share's queries are on their way while this one's sums are joined
-                now.Next(p, kv_groups);
-                share_first = 0;
-                head0 = now.kvg * p.step_heads * p.group + now.row_tile * kRows;
-                rows = min(kRows, p.group - now.row_tile * kRows);
-                load_queries(now.b, head0, rows);
-            }
             __syncthreads();
             const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (begins_run ? 0 : 1)) * p.step_heads * kRows;
-            for (int32_t i = tid; i < p.step_heads * of_rows * (kDim / 2); i += kAttendThreads) {
-                const int32_t head_row = i / (kDim / 2), kv_i = head_row / of_rows, row = head_row - kv_i * of_rows;
+            for (int32_t i = tid; i < p.step_heads * rows * (kDim / 2); i += kAttendThreads) {
+                const int32_t head_row = i / (kDim / 2), kv_i = head_row / rows, row = head_row - kv_i * rows;
                 const int32_t d = (i - head_row * (kDim / 2)) * 2;
                 float m = -INFINITY;
                 for (int32_t w = kv_i * token_tiles; w < (kv_i + 1) * token_tiles; ++w) m = fmaxf(m, join_ml[w][row].x);
@@ -586,14 +609,14 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
                 }
                 if (whole) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const int64_t head_at = static_cast<int64_t>(of_b) * p.n_q_heads + of_head0 + kv_i * p.group + row;
+                    const int64_t head_at = static_cast<int64_t>(now.b) * p.n_q_heads + head0 + kv_i * p.group + row;
                     if (d < p.pools.head_dim) {
                         T *to = reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim + d;
                         *reinterpret_cast<typename Half16<T>::Pair *>(to) = Half16<T>::FromFloat2(acc.x * inv, acc.y * inv);
                     }
                     if (d == 0) {
                         if (kScores) p.whole_ml[head_at] = make_float2(m, l);
-                        if (p.lse != nullptr) p.lse[head_at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+                        if (p.lse != nullptr) p.lse[head_at] = l == 0.0f ? -INFINITY : (m + Log2(l)) * kLn2;
                     }
                 } else {
                     const int64_t to = slot + kv_i * kRows + row;
@@ -602,10 +625,10 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim>::kCtasPerSm)
                 }
             }
             __syncthreads();  // the sums may be overwritten
-            clear();
-        } else {
-            now.Next(p, kv_groups);
+            fresh = true;
+            share_first = 0;
         }
+        if (more) now.Next(p, kv_groups);
         stage = stage + 1 == kStages ? 0 : stage + 1;
     }
     CopyWait<0>();
@@ -622,8 +645,8 @@ __device__ __forceinline__ Shares SharesAt(int64_t t0, int64_t steps, int64_t pe
     Shares s;
     s.t0 = t0;
     s.per = per;
-    s.first = static_cast<int32_t>(t0 / per);
-    s.last = static_cast<int32_t>((t0 + steps - 1) / per);
+    s.first = static_cast<int32_t>(Divide(t0, per));
+    s.last = static_cast<int32_t>(Divide(t0 + steps - 1, per));
     return s;
 }
 
@@ -653,19 +676,27 @@ struct Partial {
 //
 // Weights: the steps of all sequences and weight heads are cut into equal runs again.
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kJoinThreads, 4) JoinSharesKernel(const AttendParams p, int32_t weight_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 2) JoinSharesKernel(const __grid_constant__ AttendParams p, int32_t weight_blocks) {
     __shared__ Partial partials[kJoinThreads / 32];
-    __shared__ int32_t found_b;
+    __shared__ int64_t scan_warp[kJoinThreads / 32];
+    __shared__ Place64 found;
     extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count for a weight head
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const int64_t all = p.steps_before[p.batch];
-    const int64_t per = StepsPerRun(all * p.units, p.workers);
+    // Where this block's work lies follows from the lengths, before the first kernel is done.
+    const StepScan scan = ScanSteps<kJoinThreads>(p, scan_warp);
+    const int64_t per = StepsPerRun(scan.all * p.units, p.workers);
     if (blockIdx.x < static_cast<uint32_t>(p.workers)) {
         const int32_t w = blockIdx.x;
-        const int4 run = p.runs[w];
-        if (run.z == 0) return;
-        const int64_t steps = p.steps_before[run.x + 1] - p.steps_before[run.x];
+        if (w * per >= scan.all * p.units) return;
+        FindStep(p, scan, p.units, w * per, &found);
+        const int64_t inside = w * per - found.before;
+        int4 run;  // sequence, unit, step within the unit
+        run.x = found.b;
+        const int32_t steps = SpanOf(p, run.x).steps;
+        run.y = static_cast<int32_t>(Divide(inside, steps));
+        run.z = static_cast<int32_t>(inside - static_cast<int64_t>(run.y) * steps);
+        if (run.z == 0) return;  // nothing is cut here
+        asm volatile("griddepcontrol.wait;\n" ::: "memory");
         const Shares sh = SharesAt(w * per - run.z, steps, per);
         const int32_t cuts = sh.last - sh.first, cut = w - sh.first - 1;
         const int32_t kvg = run.y / p.row_tiles, row_tile = run.y - kvg * p.row_tiles;
@@ -720,7 +751,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) JoinSharesKernel(const Attend
                     to[0] = Half16<T>::FromFloat2(acc.o.x * inv, acc.o.y * inv);
                     to[1] = Half16<T>::FromFloat2(acc.o.z * inv, acc.o.w * inv);
                 }
-                if (d == 0 && p.lse != nullptr) p.lse[head_at] = acc.l == 0.0f ? -INFINITY : acc.m * kLn2 + logf(acc.l);
+                if (d == 0 && p.lse != nullptr) p.lse[head_at] = acc.l == 0.0f ? -INFINITY : (acc.m + Log2(acc.l)) * kLn2;
             }
         }
         return;
@@ -728,36 +759,35 @@ __global__ void __launch_bounds__(kJoinThreads, 4) JoinSharesKernel(const Attend
 
     // ---- weights: steps [at, end) of the batch's steps times weight heads
     const int32_t block = blockIdx.x - p.workers;
-    const int64_t total = all * p.n_weight_heads;
-    const int64_t share = (total + weight_blocks - 1) / weight_blocks;
+    const int64_t total = scan.all * p.n_weight_heads;
+    const int64_t share = Divide(total + weight_blocks - 1, weight_blocks);
     int64_t at = block * share;
     const int64_t end = min(total, at + share);
     if (at >= end) return;
-    for (int32_t b = tid; b < p.batch; b += kJoinThreads) {
-        if (p.steps_before[b] * p.n_weight_heads <= at && at < p.steps_before[b + 1] * p.n_weight_heads) found_b = b;
-    }
-    __syncthreads();
-    int32_t b = found_b;
+    FindStep(p, scan, p.n_weight_heads, at, &found);
+    int32_t b = found.b;
+    int64_t before = found.before;  // of sequence b, all weight heads counted
     const int32_t n_heads = p.n_weight_heads == 1 ? p.n_q_heads : p.group;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     while (at < end) {
         const Span span = SpanOf(p, b);
         if (span.steps == 0) {
             ++b;
             continue;
         }
-        const int64_t before = p.steps_before[b];
-        const int64_t inside = at - before * p.n_weight_heads;
-        const int32_t wh = static_cast<int32_t>(inside / span.steps);
+        const int64_t inside = at - before;
+        const int32_t wh = static_cast<int32_t>(Divide(inside, span.steps));
         const int32_t step0 = static_cast<int32_t>(inside - static_cast<int64_t>(wh) * span.steps);
         const int32_t steps = static_cast<int32_t>(min(static_cast<int64_t>(span.steps - step0), end - at));
         const int32_t head0 = p.n_weight_heads == 1 ? 0 : wh * p.group;
+        const int64_t unit0 = Divide(before, p.n_weight_heads) * p.units;  // first step of the sequence, all units counted
         __syncthreads();
         for (int32_t i = warp; i < n_heads; i += kJoinThreads / 32) {
             const int32_t head = head0 + i;
             const int32_t kv = head / p.group, in_group = head - kv * p.group;
             const int32_t kvg = kv / p.step_heads, kv_i = kv - kvg * p.step_heads;
             const int64_t unit = static_cast<int64_t>(kvg) * p.row_tiles + in_group / kRows;
-            const Shares sh = SharesAt(before * p.units + unit * span.steps, span.steps, per);
+            const Shares sh = SharesAt(unit0 + unit * span.steps, span.steps, per);
             float m = -INFINITY, l = 0.0f;
             if (sh.first == sh.last) {
                 const float2 ml = p.whole_ml[static_cast<int64_t>(b) * p.n_q_heads + head];
@@ -807,14 +837,17 @@ __global__ void __launch_bounds__(kJoinThreads, 4) JoinSharesKernel(const Attend
             }
         }
         at += steps;
-        if (at == (before + span.steps) * p.n_weight_heads) ++b;
+        if (at == before + static_cast<int64_t>(span.steps) * p.n_weight_heads) {
+            before = at;
+            ++b;
+        }
     }
 }
 
 int64_t Aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 struct AttendWorkspace {
-    int64_t steps_before, runs, part_o, part_ml, whole_ml, scores, total;
+    int64_t part_o, part_ml, whole_ml, scores, total;
     int64_t score_stride;
 };
 
@@ -822,9 +855,7 @@ AttendWorkspace LayOut(int32_t batch, int32_t n_q_heads, int32_t group, int32_t 
     const int rows = group <= 8 ? 8 : 16;
     const int dim = head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256);
     AttendWorkspace w;
-    w.steps_before = 0;
-    w.runs = Aligned((static_cast<int64_t>(batch) + 1) * 8);
-    w.part_o = w.runs + Aligned(int64_t{kMaxWorkers} * 16);
+    w.part_o = 0;
     w.part_ml = w.part_o + Aligned(int64_t{kMaxWorkers} * 2 * kAttendWarps * rows * dim * 4);
     w.whole_ml = w.part_ml + Aligned(int64_t{kMaxWorkers} * 2 * kAttendWarps * rows * 8);
     w.scores = w.whole_ml + (with_weights ? Aligned(static_cast<int64_t>(batch) * n_q_heads * 8) : 0);
@@ -836,7 +867,7 @@ AttendWorkspace LayOut(int32_t batch, int32_t n_q_heads, int32_t group, int32_t 
 
 template <typename T, int kDim, int kRows, bool kScores>
 void LaunchAttend(AttendParams p, cudaStream_t stream) {
-    using Shape = AttendShape<kDim>;
+    using Shape = AttendShape<kDim, kScores>;
     static_assert((Shape::kRingBytes + 2048) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
     auto *main_kernel = AttendPagesKernel<T, kDim, kRows, kScores>;
     auto *join_kernel = JoinSharesKernel<T, kDim, kRows>;
@@ -846,7 +877,7 @@ void LaunchAttend(AttendParams p, cudaStream_t stream) {
     main_kernel<<<p.workers, kAttendThreads, Shape::kRingBytes, stream>>>(p);
 
     // The second kernel's blocks wait on the device for the first kernel's end, their launch overlaps it.
-    const int32_t weight_blocks = kScores ? 8 * sm_count : 0;
+    const int32_t weight_blocks = kScores ? 2 * sm_count : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.workers + weight_blocks);
     cfg.blockDim = dim3(kJoinThreads);
@@ -944,8 +975,6 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.wo_batch = wo_batch_stride;
     p.wo_head = wo_head_stride;
     p.n_weight_heads = with_weights ? n_weight_heads : 0;
-    p.steps_before = reinterpret_cast<int64_t *>(ws + w.steps_before);
-    p.runs = reinterpret_cast<int4 *>(ws + w.runs);
     p.part_o = reinterpret_cast<float *>(ws + w.part_o);
     p.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml);
     p.whole_ml = reinterpret_cast<float2 *>(ws + w.whole_ml);
