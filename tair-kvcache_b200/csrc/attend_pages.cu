@@ -33,7 +33,7 @@ constexpr int kTile = 16;                                  // tokens of a tile
 constexpr int64_t kMinRun = 1;                             // steps of a run
 constexpr int kMaxWorkers = 512;
 constexpr int kMaxAttendHeadDim = 256;
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 128;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -667,47 +667,60 @@ struct Partial {
     }
 };
 
+// Running maximum and sum over shares [from, to] of a head, every `by`-th.
+__device__ __forceinline__ float2 StatsOf(const AttendParams &p, const Shares &sh, int32_t kv_i, int32_t row, int32_t rows,
+                                          int32_t from, int32_t by) {
+    float m = -INFINITY, l = 0.0f;
+    for (int32_t w = from; w <= sh.last; w += by) {
+        const float2 ml = __ldcg(p.part_ml + (sh.Slot(w) * p.step_heads + kv_i) * rows + row);
+        const float grown = fmaxf(m, ml.x);
+        const float use = grown == -INFINITY ? 0.0f : grown;
+        l = l * Exp2(m - use) + ml.y * Exp2(ml.x - use);
+        m = grown;
+    }
+    return make_float2(m, l);
+}
+
 // Joins the shares of heads that were cut and, in the blocks behind those, adds the attention every token received to its
-// weight.
+// weight.  It starts when the first kernel's last CTA ends, so what counts is the chain of dependent loads after that:
+// small blocks, all resident at once, find their work from the lengths while the first kernel still runs, and load all
+// they need of its results together.
 //
 // Join: block w looks at the point where run w begins.  When that lies within a unit, the unit's shares are joined by
 // the blocks of all such points together: with c cuts each block takes a c-th of the unit's output elements, four to a
 // thread group, over all shares, so that one long head is joined by as many blocks as computed it.
 //
 // Weights: the steps of all sequences and weight heads are cut into equal runs again.
-template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kJoinThreads, 2) JoinSharesKernel(const __grid_constant__ AttendParams p, int32_t weight_blocks) {
+template <typename T, int kDim, int kRows, bool kScores>
+__global__ void __launch_bounds__(kJoinThreads, 8) JoinSharesKernel(const __grid_constant__ AttendParams p, int32_t weight_blocks) {
     __shared__ Partial partials[kJoinThreads / 32];
     __shared__ int64_t scan_warp[kJoinThreads / 32];
     __shared__ Place64 found;
-    extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count for a weight head
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // Where this block's work lies follows from the lengths, before the first kernel is done.
     const StepScan scan = ScanSteps<kJoinThreads>(p, scan_warp);
     const int64_t per = StepsPerRun(scan.all * p.units, p.workers);
     if (blockIdx.x < static_cast<uint32_t>(p.workers)) {
         const int32_t w = blockIdx.x;
         if (w * per >= scan.all * p.units) return;
         FindStep(p, scan, p.units, w * per, &found);
+        const int32_t b = found.b;
+        const int32_t steps = SpanOf(p, b).steps;
         const int64_t inside = w * per - found.before;
-        int4 run;  // sequence, unit, step within the unit
-        run.x = found.b;
-        const int32_t steps = SpanOf(p, run.x).steps;
-        run.y = static_cast<int32_t>(Divide(inside, steps));
-        run.z = static_cast<int32_t>(inside - static_cast<int64_t>(run.y) * steps);
-        if (run.z == 0) return;  // nothing is cut here
-        asm volatile("griddepcontrol.wait;\n" ::: "memory");
-        const Shares sh = SharesAt(w * per - run.z, steps, per);
+        const int32_t unit = static_cast<int32_t>(Divide(inside, steps));
+        const int64_t into = inside - static_cast<int64_t>(unit) * steps;
+        if (into == 0) return;  // nothing is cut here
+        const Shares sh = SharesAt(w * per - into, steps, per);
         const int32_t cuts = sh.last - sh.first, cut = w - sh.first - 1;
-        const int32_t kvg = run.y / p.row_tiles, row_tile = run.y - kvg * p.row_tiles;
+        const int32_t kvg = unit / p.row_tiles, row_tile = unit - kvg * p.row_tiles;
         const int32_t rows = min(kRows, p.group - row_tile * kRows);
-        const int64_t head0 = static_cast<int64_t>(run.x) * p.n_q_heads + kvg * p.step_heads * p.group + row_tile * kRows;
+        const int64_t head0 = static_cast<int64_t>(b) * p.n_q_heads + kvg * p.step_heads * p.group + row_tile * kRows;
         const int32_t fours = p.step_heads * rows * (kDim / 4);    // groups of four output elements
         const int32_t mine = (fours + cuts - 1) / cuts;            // this block's
         int32_t lanes = 1;                                         // thread groups per pass, a power of two
         while (lanes < mine && lanes < kJoinThreads) lanes *= 2;
         const int32_t parts = kJoinThreads / lanes;                // threads that share a group's shares
         const int32_t at = tid / parts, part = tid % parts;
+        asm volatile("griddepcontrol.wait;\n" ::: "memory");
         for (int32_t base = 0; base < mine; base += lanes) {
             const int32_t four = cut * mine + base + at;
             const bool live = base + at < mine && four < fours;
@@ -715,13 +728,21 @@ __global__ void __launch_bounds__(kJoinThreads, 2) JoinSharesKernel(const __grid
             const int32_t kv_i = head_row / rows, row = head_row - kv_i * rows;
             const int64_t head_at = head0 + kv_i * p.group + row;
             Partial acc = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-            if (live) {
-#pragma unroll 4
-                for (int32_t i = sh.first + part; i <= sh.last; i += parts) {
-                    const int64_t slot = (sh.Slot(i) * p.step_heads + kv_i) * kRows + row;
-                    const float2 ml = __ldcg(p.part_ml + slot);
-                    acc.Add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d)));
+            constexpr int kTogether = 4;
+            for (int32_t i0 = sh.first + part; live && i0 <= sh.last; i0 += kTogether * parts) {
+                Partial got[kTogether];
+#pragma unroll
+                for (int j = 0; j < kTogether; ++j) {
+                    const int32_t i = i0 + j * parts;
+                    got[j] = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+                    if (i <= sh.last) {
+                        const int64_t slot = (sh.Slot(i) * p.step_heads + kv_i) * kRows + row;
+                        const float2 ml = __ldcg(p.part_ml + slot);
+                        got[j] = {ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d))};
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < kTogether; ++j) acc.Add(got[j].m, got[j].l, got[j].o);
             }
             for (int32_t i = 1; i < min(parts, 32); i *= 2) {
                 Partial other;
@@ -756,8 +777,10 @@ __global__ void __launch_bounds__(kJoinThreads, 2) JoinSharesKernel(const __grid
         }
         return;
     }
+    if (!kScores) return;
 
     // ---- weights: steps [at, end) of the batch's steps times weight heads
+    extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count for a weight head
     const int32_t block = blockIdx.x - p.workers;
     const int64_t total = scan.all * p.n_weight_heads;
     const int64_t share = Divide(total + weight_blocks - 1, weight_blocks);
@@ -781,59 +804,85 @@ __global__ void __launch_bounds__(kJoinThreads, 2) JoinSharesKernel(const __grid
         const int32_t steps = static_cast<int32_t>(min(static_cast<int64_t>(span.steps - step0), end - at));
         const int32_t head0 = p.n_weight_heads == 1 ? 0 : wh * p.group;
         const int64_t unit0 = Divide(before, p.n_weight_heads) * p.units;  // first step of the sequence, all units counted
-        __syncthreads();
-        for (int32_t i = warp; i < n_heads; i += kJoinThreads / 32) {
-            const int32_t head = head0 + i;
-            const int32_t kv = head / p.group, in_group = head - kv * p.group;
-            const int32_t kvg = kv / p.step_heads, kv_i = kv - kvg * p.step_heads;
-            const int64_t unit = static_cast<int64_t>(kvg) * p.row_tiles + in_group / kRows;
-            const Shares sh = SharesAt(unit0 + unit * span.steps, span.steps, per);
-            float m = -INFINITY, l = 0.0f;
-            if (sh.first == sh.last) {
-                const float2 ml = p.whole_ml[static_cast<int64_t>(b) * p.n_q_heads + head];
-                m = ml.x;
-                l = ml.y;
-            } else {
-                for (int32_t w = sh.first + lane; w <= sh.last; w += 32) {
-                    const float2 ml = __ldcg(p.part_ml + (sh.Slot(w) * p.step_heads + kv_i) * kRows + in_group % kRows);
-                    const float grown = fmaxf(m, ml.x);
-                    const float use = grown == -INFINITY ? 0.0f : grown;
-                    l = l * Exp2(m - use) + ml.y * Exp2(ml.x - use);
-                    m = grown;
-                }
-#pragma unroll
-                for (int d = 16; d > 0; d /= 2) {
-                    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
-                    const float grown = fmaxf(m, m2);
-                    const float use = grown == -INFINITY ? 0.0f : grown;
-                    l = l * Exp2(m - use) + l2 * Exp2(m2 - use);
-                    m = grown;
-                }
-            }
-            if (lane == 0) head_ml[i] = make_float2(m == -INFINITY ? 0.0f : m, l == 0.0f ? 0.0f : 1.0f / l);
-        }
-        __syncthreads();
+        // Where the shares of head0 + i lie, and its KV head and row in them.
+        auto shares_of = [&](int32_t i, int32_t &kv_i, int32_t &row) {
+            const int32_t kv = (head0 + i) / p.group, in_group = head0 + i - kv * p.group;
+            const int32_t kvg = kv / p.step_heads;
+            kv_i = kv - kvg * p.step_heads;
+            row = in_group % kRows;
+            return SharesAt(unit0 + (static_cast<int64_t>(kvg) * p.row_tiles + in_group / kRows) * span.steps, span.steps, per);
+        };
         // a token on a page outside the pool was masked like any other: its score is negative infinity
         const float *scores = p.scores + (static_cast<int64_t>(b) * p.n_q_heads + head0) * p.score_stride;
         const float *w_in = p.weights + b * p.w_batch + wh * p.w_head;
         float *w_out = p.weights_out + b * p.wo_batch + wh * p.wo_head;
-        const int32_t last = min((step0 + steps) * p.step_tokens, span.len - span.base);  // relative to the span's base
-        constexpr int kAtOnce = 4;  // tokens of a thread, whose loads are in flight together
-        for (int32_t t0 = step0 * p.step_tokens + static_cast<int32_t>(tid); t0 < last; t0 += kAtOnce * kJoinThreads) {
-            float received[kAtOnce] = {};
-#pragma unroll 2
-            for (int32_t i = 0; i < n_heads; ++i) {
-                const float2 ml = head_ml[i];
-                const float *row = scores + i * p.score_stride + t0;
+        const int32_t t_begin = step0 * p.step_tokens;  // relative to the span's base, as `last`
+        const int32_t last = min((step0 + steps) * p.step_tokens, span.len - span.base);
+        constexpr int kAtOnce = 4, kHeadsAtOnce = 4;  // tokens and heads of a thread whose loads are in flight together
+        for (int32_t t_block = t_begin; t_block < last; t_block += kAtOnce * kJoinThreads) {
+            const int32_t t0 = t_block + static_cast<int32_t>(tid);
+            float received[kAtOnce] = {}, old[kAtOnce] = {};
+            for (int32_t i0 = 0; i0 < n_heads; i0 += kHeadsAtOnce) {
+                float score[kHeadsAtOnce][kAtOnce];
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    if (t0 + j * kJoinThreads < last) received[j] += Exp2(__ldcg(row + j * kJoinThreads) - ml.x) * ml.y;
+                for (int h = 0; h < kHeadsAtOnce; ++h) {
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        score[h][j] = -INFINITY;
+                        if (i0 + h < n_heads && t0 + j * kJoinThreads < last) {
+                            score[h][j] = __ldcg(scores + (i0 + h) * p.score_stride + t0 + j * kJoinThreads);
+                        }
+                    }
+                }
+                if (i0 == 0) {
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        const int32_t t = span.base + t0 + j * kJoinThreads;
+                        if (t0 + j * kJoinThreads < last && t >= span.first) old[j] = w_in[t];
+                    }
+                    if (t_block == t_begin) {
+                        // maximum and sum of every head that counts here, of few shares by a thread, of many by a warp
+                        __syncthreads();
+                        const int32_t by = span.steps > 6 * per ? 32 : 1;
+                        for (int32_t i = static_cast<int32_t>(tid) / by; i < n_heads; i += kJoinThreads / by) {
+                            int32_t kv_i, row;
+                            const Shares sh = shares_of(i, kv_i, row);
+                            float2 ml;
+                            if (sh.first == sh.last) {
+                                ml = __ldcg(p.whole_ml + static_cast<int64_t>(b) * p.n_q_heads + head0 + i);
+                            } else {
+                                ml = StatsOf(p, sh, kv_i, row, kRows, sh.first + static_cast<int32_t>(tid) % by, by);
+                            }
+                            if (by == 32 && sh.first != sh.last) {
+#pragma unroll
+                                for (int d = 16; d > 0; d /= 2) {
+                                    const float m2 = __shfl_xor_sync(0xffffffffu, ml.x, d), l2 = __shfl_xor_sync(0xffffffffu, ml.y, d);
+                                    const float grown = fmaxf(ml.x, m2);
+                                    const float use = grown == -INFINITY ? 0.0f : grown;
+                                    ml.y = ml.y * Exp2(ml.x - use) + l2 * Exp2(m2 - use);
+                                    ml.x = grown;
+                                }
+                            }
+                            if (tid % by == 0) {
+                                head_ml[i] = make_float2(ml.x == -INFINITY ? 0.0f : ml.x, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
+                            }
+                        }
+                        __syncthreads();
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < kHeadsAtOnce; ++h) {
+                    if (i0 + h < n_heads) {
+                        const float2 ml = head_ml[i0 + h];
+#pragma unroll
+                        for (int j = 0; j < kAtOnce; ++j) received[j] += Exp2(score[h][j] - ml.x) * ml.y;
+                    }
                 }
             }
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
                 const int32_t t = span.base + t0 + j * kJoinThreads;
-                if (t0 + j * kJoinThreads < last && t >= span.first) w_out[t] = w_in[t] + received[j];
+                if (t0 + j * kJoinThreads < last && t >= span.first) w_out[t] = old[j] + received[j];
             }
         }
         at += steps;
@@ -870,14 +919,14 @@ void LaunchAttend(AttendParams p, cudaStream_t stream) {
     using Shape = AttendShape<kDim, kScores>;
     static_assert((Shape::kRingBytes + 2048) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
     auto *main_kernel = AttendPagesKernel<T, kDim, kRows, kScores>;
-    auto *join_kernel = JoinSharesKernel<T, kDim, kRows>;
+    auto *join_kernel = JoinSharesKernel<T, kDim, kRows, kScores>;
     EnsureDynamicSmem(main_kernel, Shape::kRingBytes);
     const int32_t sm_count = GetDeviceInfo().sm_count;
     p.workers = std::min(kMaxWorkers, sm_count * Shape::kCtasPerSm);
     main_kernel<<<p.workers, kAttendThreads, Shape::kRingBytes, stream>>>(p);
 
     // The second kernel's blocks wait on the device for the first kernel's end, their launch overlaps it.
-    const int32_t weight_blocks = kScores ? 2 * sm_count : 0;
+    const int32_t weight_blocks = kScores ? 5 * sm_count : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.workers + weight_blocks);
     cfg.blockDim = dim3(kJoinThreads);
