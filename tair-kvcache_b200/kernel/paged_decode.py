@@ -70,17 +70,26 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
     return freq.to(torch.float32).to(device), attention_factor
 
 
-def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor):
-    """The fields of kvcm_b200_kv_pools_t."""
-    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride():
+# Layouts are checked once and remembered by what they are - shapes, strides, types, devices, never addresses - so that a
+# decode loop, which calls with the same ones over and over, pays for a dictionary lookup.
+_REMEMBERED = 1024
+
+
+def _layout(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _pools(k, v):
+    """The fields of kvcm_b200_kv_pools_t behind the two addresses, from the pools' layouts."""
+    (shape, strides, dtype, device) = k
+    if len(shape) != 4 or v[0] != shape or v[1] != strides:
         raise ValueError("the K and V pools must be [pages, page_tokens, heads, dim] tensors of one shape and layout")
-    dtype = _DTYPES.get(k_pool.dtype)
-    if dtype is None or v_pool.dtype != k_pool.dtype:
-        raise ValueError("the pools must hold bfloat16 or float16, got %s and %s" % (k_pool.dtype, v_pool.dtype))
-    if not k_pool.is_cuda or v_pool.device != k_pool.device:
+    if dtype not in _DTYPES or v[2] != dtype:
+        raise ValueError("the pools must hold bfloat16 or float16, got %s and %s" % (dtype, v[2]))
+    if device.type != "cuda" or v[3] != device:
         raise ValueError("the pools must live on one GPU")
-    pages, page_tokens, heads, dim = k_pool.shape
-    sp, st, sh, se = k_pool.stride()
+    pages, page_tokens, heads, dim = shape
+    sp, st, sh, se = strides
     if page_tokens == 0 or heads == 0 or dim == 0:
         raise ValueError("the pools' pages are empty")
     if se != 1 and dim > 1:
@@ -89,68 +98,118 @@ def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor):
     sp, st, sh = sp if pages > 1 else 0, st if page_tokens > 1 else 0, sh if heads > 1 else 0
     if (pages > 1 and sp == 0) or (page_tokens > 1 and st == 0) or (heads > 1 and sh == 0):
         raise ValueError("rows of the pools share memory")
-    return (k_pool.data_ptr(), v_pool.data_ptr(), pages, sp, st, sh, page_tokens, heads, dim, dtype)
+    return (pages, sp, st, sh, page_tokens, heads, dim, _DTYPES[dtype])
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("the paged decode operators have no gradient: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("the paged decode operators have no gradient: call them under torch.no_grad()")
 
 
-def _heads(t: torch.Tensor, name: str, pool: torch.Tensor, count: int):
-    if t.dim() != 3 or t.shape[0] != count or t.shape[2] != pool.shape[3]:
-        raise ValueError("%s must be [%d, heads, %d], got %s" % (name, count, pool.shape[3], list(t.shape)))
-    if t.dtype != pool.dtype or t.device != pool.device:
+def _heads(t, name: str, pool, count: int):
+    """A layout of [count, heads, dim] beside a pool's; the strides between tokens and heads, and the number of heads."""
+    shape, strides, dtype, device = t
+    if len(shape) != 3 or shape[0] != count or shape[2] != pool[0][3]:
+        raise ValueError("%s must be [%d, heads, %d], got %s" % (name, count, pool[0][3], list(shape)))
+    if dtype != pool[2] or device != pool[3]:
         raise ValueError("%s must have the pools' type and device" % name)
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    if strides[2] != 1 and shape[2] > 1:
         raise ValueError("the elements of a head must be contiguous in %s" % name)
-    return t
+    return strides[0], strides[1], shape[1]
 
 
-def _own_rows(t: torch.Tensor, name: str):
+def _own_rows(t, name: str):
     """A tensor that is written: no two of its rows may be the same memory."""
-    for size, stride in zip(t.shape, t.stride()):
+    for size, stride in zip(t[0], t[1]):
         if size > 1 and stride == 0:
             raise ValueError("rows of %s share memory" % name)
-    return t
 
 
-def _sequences(block_table: torch.Tensor, context_lens: torch.Tensor, pool: torch.Tensor):
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != pool.device:
+def _contiguous(t) -> bool:
+    expected = 1
+    for size, stride in zip(reversed(t[0]), reversed(t[1])):
+        if size != 1 and stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _sequences(table, lens, pool):
+    """Number of sequences, pages per sequence and the stride between sequences of the table."""
+    if len(table[0]) != 2 or table[2] != torch.int32 or table[3] != pool[3]:
         raise ValueError("block_table must be an int32 [sequences, pages] tensor on the pools' device")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+    if table[1][1] != 1 and table[0][1] > 1:
         raise ValueError("the pages of a sequence must be contiguous in block_table")
-    if (context_lens.dim() != 1 or context_lens.dtype != torch.int32 or context_lens.device != pool.device or
-            context_lens.shape[0] != block_table.shape[0] or not context_lens.is_contiguous()):
+    if len(lens[0]) != 1 or lens[2] != torch.int32 or lens[3] != pool[3] or lens[0][0] != table[0][0] or not _contiguous(lens):
         raise ValueError("context_lens must be a contiguous int32 [sequences] tensor on the pools' device")
-    return block_table.shape[0], block_table.shape[1]
+    return table[0][0], table[0][1], table[1][0]
 
 
-def _per_slot(t: torch.Tensor, name: str, dtype: torch.dtype, pool: torch.Tensor, batch: int, tokens: int, heads=None):
-    if (t.dim() != 3 or t.dtype != dtype or t.device != pool.device or t.shape[0] != batch or t.shape[2] < tokens or
-            t.shape[1] not in ((1, pool.shape[2]) if heads is None else (heads,)) or (t.stride(2) != 1 and t.shape[2] > 1)):
+def _per_slot(t, name: str, dtype: torch.dtype, pool, batch: int, tokens: int, heads=None):
+    """Strides between sequences and heads, and the number of heads, of an array with an entry per slot."""
+    shape, strides = t[0], t[1]
+    if (len(shape) != 3 or t[2] != dtype or t[3] != pool[3] or shape[0] != batch or shape[2] < tokens or
+            shape[1] not in ((1, pool[0][2]) if heads is None else (heads,)) or (strides[2] != 1 and shape[2] > 1)):
         raise ValueError("%s must be a %s [%d, %s, >= %d] tensor on the pools' device, contiguous along the last axis, "
                          "with an entry for every token of the block table"
-                         % (name, dtype, batch, "1 or %d" % pool.shape[2] if heads is None else heads, tokens))
-    return t
+                         % (name, dtype, batch, "1 or %d" % pool[0][2] if heads is None else heads, tokens))
+    return strides[0], strides[1], shape[1]
 
 
-def _status_ptr(status: Optional[torch.Tensor], pool: torch.Tensor) -> int:
+def _status_ptr(status: Optional[torch.Tensor], device: torch.device) -> int:
     if status is None:
         return 0
-    if status.numel() < 4 or status.element_size() != 4 or status.device != pool.device or not status.is_contiguous():
+    if status.numel() < 4 or status.element_size() != 4 or status.device != device or not status.is_contiguous():
         raise ValueError("status must be four 32-bit words on the pools' device")
     return status.data_ptr()
 
 
 def _launch(name: str, device: torch.device, pools, *args) -> None:
-    _cabi.bind_device(device.index)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    index = device.index
+    _cabi.bind_device(index)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
         _cabi.call_pages(name, pools, *args, stream)
     else:
         with torch.cuda.device(device):
             _cabi.call_pages(name, pools, *args, stream)
+
+
+def _workspace_bytes(name: str, size: int) -> int:
+    if size < 0:
+        raise _cabi.KvcmError(_cabi.KVCM_EC_OUT_OF_LIMIT, name)
+    return size
+
+
+@functools.lru_cache(maxsize=_REMEMBERED)
+def _append_plan(query, key, value, positions, slots, k, v, inv_freq, query_out):
+    pools = _pools(k, v)
+    tokens = key[0][0] if len(key[0]) else 0
+    k_args, v_args = _heads(key, "key", k, tokens), _heads(value, "value", k, tokens)
+    if k_args[2] != pools[5] or v_args[2] != pools[5]:
+        raise ValueError("key and value must have the pools' %d heads" % pools[5])
+    for t, name in ((positions, "positions"), (slots, "slot_indices")):
+        if len(t[0]) != 1 or t[2] not in _INDEX_BYTES or t[0][0] != tokens or t[3] != k[3] or not _contiguous(t):
+            raise ValueError("%s must be a contiguous int32 or int64 [%d] tensor on the pools' device" % (name, tokens))
+    if len(inv_freq[0]) != 1 or inv_freq[2] != torch.float32 or inv_freq[3] != k[3] or not _contiguous(inv_freq) or (
+            2 * inv_freq[0][0] > pools[6]):
+        raise ValueError("inv_freq must be a contiguous float32 tensor of at most dim / 2 frequencies on the pools' device")
+    q_args = q_out_args = None
+    if query is not None:
+        q_args = _heads(query, "query", k, tokens)
+        if query_out is None:
+            q_out_args = (q_args[2] * pools[6], pools[6])
+        else:
+            if query_out[0] != query[0]:
+                raise ValueError("query_out must have query's shape")
+            q_out_args = _heads(query_out, "query_out", k, tokens)[:2]
+            _own_rows(query_out, "query_out")
+    elif query_out is not None:
+        raise ValueError("query_out without query")
+    return (pools, tokens, q_args, q_out_args, k_args[:2], v_args[:2], _INDEX_BYTES[positions[2]], _INDEX_BYTES[slots[2]],
+            2 * inv_freq[0][0], k[3])
 
 
 def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, value: torch.Tensor,
@@ -168,54 +227,48 @@ def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, valu
     nothing; any other slot outside the pool is skipped and counted in `status` (four zeroed 32-bit words on the GPU).
     The same slot twice in one call is a data race.  `query_out` may be `query`."""
     _no_grad(query, key, value, inv_freq)
-    pools = _pools(k_pool, v_pool)
-    tokens = key.shape[0] if key.dim() else 0
-    _heads(key, "key", k_pool, tokens)
-    _heads(value, "value", k_pool, tokens)
-    if key.shape[1] != k_pool.shape[2] or value.shape[1] != k_pool.shape[2]:
-        raise ValueError("key and value must have the pools' %d heads" % k_pool.shape[2])
     if not isinstance(slot_indices, torch.Tensor):
         slot_indices = _index_tensor(slot_indices, k_pool.device)
-    for t, name in ((positions, "positions"), (slot_indices, "slot_indices")):
-        if (t.dim() != 1 or t.dtype not in _INDEX_BYTES or t.shape[0] != tokens or t.device != k_pool.device or
-                not t.is_contiguous()):
-            raise ValueError("%s must be a contiguous int32 or int64 [%d] tensor on the pools' device" % (name, tokens))
-    if (inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or inv_freq.device != k_pool.device or
-            not inv_freq.is_contiguous() or 2 * inv_freq.shape[0] > k_pool.shape[3]):
-        raise ValueError("inv_freq must be a contiguous float32 tensor of at most dim / 2 frequencies on the pools' device")
-    q_args = (0, 0, 0, 0, 0, 0, 0)
-    if query is not None:
-        _heads(query, "query", k_pool, tokens)
+    pools, tokens, q_args, q_out_args, k_args, v_args, position_bytes, slot_bytes, rotary_dim, device = _append_plan(
+        _layout(query), _layout(key), _layout(value), _layout(positions), _layout(slot_indices), _layout(k_pool),
+        _layout(v_pool), _layout(inv_freq), _layout(query_out))
+    if q_args is None:
+        q_all = (0, 0, 0, 0, 0, 0, 0)
+    else:
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        elif query_out.shape != query.shape:
-            raise ValueError("query_out must have query's shape")
-        _own_rows(_heads(query_out, "query_out", k_pool, tokens), "query_out")
-        q_args = (query.data_ptr(), query.stride(0), query.stride(1), query.shape[1], query_out.data_ptr(),
-                  query_out.stride(0), query_out.stride(1))
-    elif query_out is not None:
-        raise ValueError("query_out without query")
-    _launch("kvcm_b200_append_pages", k_pool.device, pools, *q_args, key.data_ptr(), key.stride(0), key.stride(1),
-            value.data_ptr(), value.stride(0), value.stride(1), positions.data_ptr(), _INDEX_BYTES[positions.dtype],
-            slot_indices.data_ptr(), _INDEX_BYTES[slot_indices.dtype], tokens, inv_freq.data_ptr(),
-            2 * inv_freq.shape[0], int(interleaved), float(attention_factor), _status_ptr(status, k_pool))
+            query_out = query.new_empty(query.shape)
+        q_all = (query.data_ptr(), *q_args, query_out.data_ptr(), *q_out_args)
+    _launch("kvcm_b200_append_pages", device, (k_pool.data_ptr(), v_pool.data_ptr(), *pools), *q_all, key.data_ptr(), *k_args,
+            value.data_ptr(), *v_args, positions.data_ptr(), position_bytes, slot_indices.data_ptr(), slot_bytes, tokens,
+            inv_freq.data_ptr(), rotary_dim, int(interleaved), float(attention_factor), _status_ptr(status, device))
     return query_out
 
 
-@functools.lru_cache(maxsize=4096)
-def _attend_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim, tokens, with_weights):
-    return _cabi.lib().kvcm_b200_attend_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim, tokens, with_weights)
-
-
-@functools.lru_cache(maxsize=4096)
-def _evict_workspace_bytes(batch, heads, tokens, budget):
-    return _cabi.lib().kvcm_b200_evict_workspace_bytes(batch, heads, tokens, budget)
-
-
-def _workspace(size: int, device: torch.device, name: str) -> torch.Tensor:
-    if size < 0:
-        raise _cabi.KvcmError(_cabi.KVCM_EC_OUT_OF_LIMIT, name)
-    return torch.empty(size, dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=_REMEMBERED)
+def _attend_plan(query, k, v, table, lens, window, out, lse, weights, weights_out):
+    pools = _pools(k, v)
+    batch, width, table_stride = _sequences(table, lens, k)
+    q_args = _heads(query, "query", k, batch)
+    n_q_heads, n_kv_heads, dim = q_args[2], pools[5], pools[6]
+    if n_q_heads == 0 or n_q_heads % n_kv_heads:
+        raise ValueError("%d query heads are not a multiple of %d KV heads" % (n_q_heads, n_kv_heads))
+    if window < 0:
+        raise ValueError("window must not be negative")
+    if out is not None and (out[0] != query[0] or out[2:] != query[2:] or not _contiguous(out)):
+        raise ValueError("out must be contiguous, of query's shape, type and device")
+    if lse is not None and (lse[0] != query[0][:2] or lse[2] != torch.float32 or lse[3] != k[3] or not _contiguous(lse)):
+        raise ValueError("lse must be a contiguous float32 [sequences, q_heads] tensor on the pools' device")
+    tokens = width * pools[4]
+    w_args = wo_args = None
+    if weights is not None:
+        w_args = _per_slot(weights, "weights", torch.float32, k, batch, tokens)
+        wo_args = w_args if weights_out is None else _per_slot(weights_out, "weights_out", torch.float32, k, batch, tokens, w_args[2])
+        _own_rows(weights if weights_out is None else weights_out, "weights_out")
+    elif weights_out is not None:
+        raise ValueError("weights_out without weights")
+    size = _workspace_bytes("kvcm_b200_attend_pages", _cabi.lib().kvcm_b200_attend_workspace_bytes(
+        batch, n_q_heads, n_kv_heads, dim, tokens, int(weights is not None)))
+    return pools, (*q_args[:2], batch, n_q_heads), (table_stride, width), w_args, wo_args, size, dim ** -0.5, k[3]
 
 
 def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -236,41 +289,41 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     the attention each token got, summed over the query heads of its KV head or, with one weight head, over all of
     them - what batch_evict_kv_pages ranks by.  Entries that are not attended are left as they are."""
     _no_grad(query, k_pool, v_pool, weights)
-    pools = _pools(k_pool, v_pool)
-    batch, width = _sequences(block_table, context_lens, k_pool)
-    _heads(query, "query", k_pool, batch)
-    n_q_heads, n_kv_heads, dim = query.shape[1], k_pool.shape[2], k_pool.shape[3]
-    if n_q_heads == 0 or n_q_heads % n_kv_heads:
-        raise ValueError("%d query heads are not a multiple of %d KV heads" % (n_q_heads, n_kv_heads))
-    if window < 0:
-        raise ValueError("window must not be negative")
+    pools, q_args, table_args, w_args, wo_args, size, default_scale, device = _attend_plan(
+        _layout(query), _layout(k_pool), _layout(v_pool), _layout(block_table), _layout(context_lens), int(window),
+        _layout(out), _layout(lse), _layout(weights), _layout(weights_out))
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of query's shape, type and device")
-    if lse is not None and (lse.shape != query.shape[:2] or lse.dtype != torch.float32 or lse.device != query.device or
-                            not lse.is_contiguous()):
-        raise ValueError("lse must be a contiguous float32 [sequences, q_heads] tensor on the pools' device")
-    tokens = width * k_pool.shape[1]
-    w_args = (0, 0, 0, 0, 0, 0, 0)
-    if weights is not None:
-        _per_slot(weights, "weights", torch.float32, k_pool, batch, tokens)
-        if weights_out is None:
-            weights_out = weights
-        else:
-            _per_slot(weights_out, "weights_out", torch.float32, k_pool, batch, tokens, weights.shape[1])
-        _own_rows(weights_out, "weights_out")
-        w_args = (weights.data_ptr(), weights.stride(0), weights.stride(1), weights_out.data_ptr(),
-                  weights_out.stride(0), weights_out.stride(1), weights.shape[1])
-    elif weights_out is not None:
-        raise ValueError("weights_out without weights")
-    size = _attend_workspace_bytes(batch, n_q_heads, n_kv_heads, dim, tokens, int(weights is not None))
-    workspace = _workspace(size, k_pool.device, "kvcm_b200_attend_pages")
-    _launch("kvcm_b200_attend_pages", k_pool.device, pools, query.data_ptr(), query.stride(0), query.stride(1), batch,
-            n_q_heads, block_table.data_ptr(), block_table.stride(0), width, context_lens.data_ptr(),
-            dim ** -0.5 if scale is None else float(scale), int(window), out.data_ptr(),
-            0 if lse is None else lse.data_ptr(), *w_args, workspace.data_ptr(), size, _status_ptr(status, k_pool))
+        out = query.new_empty(query.shape)
+    w_all = (0, 0, 0, 0, 0, 0, 0)
+    if w_args is not None:
+        w_all = (weights.data_ptr(), *w_args[:2], (weights if weights_out is None else weights_out).data_ptr(), *wo_args)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _launch("kvcm_b200_attend_pages", device, (k_pool.data_ptr(), v_pool.data_ptr(), *pools), query.data_ptr(), *q_args,
+            block_table.data_ptr(), *table_args, context_lens.data_ptr(), default_scale if scale is None else float(scale),
+            int(window), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *w_all, workspace.data_ptr(), size,
+            _status_ptr(status, device))
     return out
+
+
+@functools.lru_cache(maxsize=_REMEMBERED)
+def _evict_plan(k, v, table, lens, weights, positions, budget, recent, weights_out, positions_out):
+    pools = _pools(k, v)
+    batch, width, table_stride = _sequences(table, lens, k)
+    tokens = width * pools[4]
+    if budget < 1 or recent < 0 or recent > budget:
+        raise ValueError("0 <= recent <= budget and budget >= 1 are needed, got recent=%r budget=%r" % (recent, budget))
+    w_args = _per_slot(weights, "weights", torch.float32, k, batch, tokens)
+    heads = w_args[2]
+    p_args = _per_slot(positions, "positions", torch.int32, k, batch, tokens, heads)
+    wo_args = w_args if weights_out is None else _per_slot(weights_out, "weights_out", torch.float32, k, batch, tokens, heads)
+    po_args = p_args if positions_out is None else _per_slot(positions_out, "positions_out", torch.int32, k, batch, tokens, heads)
+    _own_rows(weights if weights_out is None else weights_out, "weights_out")
+    _own_rows(positions if positions_out is None else positions_out, "positions_out")
+    # a budget beyond the table evicts nothing, as the table's size does
+    budget = min(budget, max(tokens, 1))
+    size = _workspace_bytes("kvcm_b200_evict_pages", _cabi.lib().kvcm_b200_evict_workspace_bytes(batch, heads, tokens, budget))
+    return (pools, (table_stride, width), batch, (budget, min(recent, budget), heads), w_args[:2], p_args[:2], wo_args[:2],
+            po_args[:2], size, k[3])
 
 
 def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -292,31 +345,14 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     Pages are packed in place: a page that two sequences share must be copied first.  A move from or to a page outside
     the pool is left out and counted in `status`, as is a length beyond the table (cut to it)."""
     _no_grad(k_pool, v_pool, weights)
-    pools = _pools(k_pool, v_pool)
-    batch, width = _sequences(block_table, context_lens, k_pool)
-    tokens = width * k_pool.shape[1]
-    if budget < 1 or recent < 0 or recent > budget:
-        raise ValueError("0 <= recent <= budget and budget >= 1 are needed, got recent=%r budget=%r" % (recent, budget))
-    _per_slot(weights, "weights", torch.float32, k_pool, batch, tokens)
-    heads = weights.shape[1]
-    _per_slot(positions, "positions", torch.int32, k_pool, batch, tokens, heads)
-    if weights_out is None:
-        weights_out = weights
-    else:
-        _per_slot(weights_out, "weights_out", torch.float32, k_pool, batch, tokens, heads)
-    if positions_out is None:
-        positions_out = positions
-    else:
-        _per_slot(positions_out, "positions_out", torch.int32, k_pool, batch, tokens, heads)
-    _own_rows(weights_out, "weights_out")
-    _own_rows(positions_out, "positions_out")
-    new_lens = torch.empty(batch, dtype=torch.int32, device=k_pool.device)
-    budget = min(int(budget), max(tokens, 1))
-    size = _evict_workspace_bytes(batch, heads, tokens, budget)
-    workspace = _workspace(size, k_pool.device, "kvcm_b200_evict_pages")
-    _launch("kvcm_b200_evict_pages", k_pool.device, pools, batch, block_table.data_ptr(), block_table.stride(0), width,
-            context_lens.data_ptr(), budget, min(int(recent), budget), heads, weights.data_ptr(), weights.stride(0),
-            weights.stride(1), positions.data_ptr(), positions.stride(0), positions.stride(1), weights_out.data_ptr(),
-            weights_out.stride(0), weights_out.stride(1), positions_out.data_ptr(), positions_out.stride(0),
-            positions_out.stride(1), new_lens.data_ptr(), workspace.data_ptr(), size, _status_ptr(status, k_pool))
+    pools, table_args, batch, sizes, w_args, p_args, wo_args, po_args, size, device = _evict_plan(
+        _layout(k_pool), _layout(v_pool), _layout(block_table), _layout(context_lens), _layout(weights), _layout(positions),
+        int(budget), int(recent), _layout(weights_out), _layout(positions_out))
+    new_lens = context_lens.new_empty(batch)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _launch("kvcm_b200_evict_pages", device, (k_pool.data_ptr(), v_pool.data_ptr(), *pools), batch, block_table.data_ptr(),
+            *table_args, context_lens.data_ptr(), *sizes, weights.data_ptr(), *w_args, positions.data_ptr(), *p_args,
+            (weights if weights_out is None else weights_out).data_ptr(), *wo_args,
+            (positions if positions_out is None else positions_out).data_ptr(), *po_args, new_lens.data_ptr(),
+            workspace.data_ptr(), size, _status_ptr(status, device))
     return new_lens

@@ -115,19 +115,29 @@ def test_workspace_sizes():
 
 
 def test_python_refuses_cpu_tensors_and_gradients():
+    layout = paged_decode._layout
     pool = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="GPU"):
-        paged_decode._pools(pool, pool.clone())
+        paged_decode._pools(layout(pool), layout(pool.clone()))
     with pytest.raises(ValueError, match="one shape"):
-        paged_decode._pools(pool, pool[:3])
+        paged_decode._pools(layout(pool), layout(pool[:3]))
     with pytest.raises(ValueError, match="bfloat16 or float16"):
-        paged_decode._pools(pool.float(), pool.float())
+        paged_decode._pools(layout(pool.float()), layout(pool.float()))
     with pytest.raises(ValueError, match="no gradient"):
         paged_decode._no_grad(torch.zeros(1, requires_grad=True))
     with torch.no_grad():
         paged_decode._no_grad(torch.zeros(1, requires_grad=True))
     with pytest.raises(ValueError, match="share memory"):
-        paged_decode._own_rows(torch.zeros(1, 1, 8).expand(2, 1, 8), "x")
+        paged_decode._own_rows(layout(torch.zeros(1, 1, 8).expand(2, 1, 8)), "x")
+
+
+def test_contiguity_of_a_layout_is_torchs():
+    layout = paged_decode._layout
+    base = torch.zeros(4, 6, 8)
+    for t in (base, base[:, :1], base[:1], base[:, ::2], base.transpose(0, 1), base[:, :, :1], base[0], base[0, :, 0], base[:0],
+              torch.zeros(1, 1).expand(3, 1), torch.zeros(3, 1).expand(3, 5)):
+        if t.numel():
+            assert paged_decode._contiguous(layout(t)) == t.is_contiguous(), (t.shape, t.stride())
 
 
 def test_rotary_frequencies():
