@@ -7,11 +7,11 @@
 // grows by one token per step, where packing in order would move up to the whole cache.
 //
 // The rank is not sorted out: the weight becomes a 32-bit key whose unsigned order is the rank, and the budget-th largest
-// key is found by counting digits (11, 11 and 10 bits) in shared memory.  One thread-block cluster takes one head of
-// one sequence; each CTA holds its slice of the keys in shared memory, and the digit counts are added up over distributed
+// key is found by counting its four bytes, from the top, in shared memory.  One CTA takes one head of one sequence, or a
+// thread-block cluster does, each CTA with a slice of the keys in shared memory and the counts added up over distributed
 // shared memory.  That kernel is a chain of short phases, bound by their latencies; it leaves a list of moves.  The
 // second kernel is bound by HBM: it spreads the moves of all heads over the whole GPU, so that one long sequence is
-// packed by every SM.  (One kernel for both left the rows of a head to the cluster that ranked it: 703 us instead of 61
+// packed by every SM.  (One kernel for both left the rows of a head to the cluster that ranked it: 703 us
 // for 131,072 slots of eight heads.)
 #include <cooperative_groups.h>
 
@@ -24,12 +24,14 @@ namespace {
 
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 256;
+constexpr int kPasses = 4;
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kKeyProtected = 0xFFFFFFFFu;
 constexpr uint32_t kKeyNan = 0xFFFFFFFEu;
-// Keys a CTA keeps in shared memory; longer slices are read again from global memory in every pass.
-constexpr int kMaxCachedKeys = 49152;
+// Slots a CTA keeps in shared memory, key and position; longer slices are read again from global memory in every pass.
+constexpr int kMaxCachedSlots = 24576;
+constexpr int kLoads = 8;  // loads of a thread in flight together
 constexpr int kMoveThreads = 256;
 constexpr int kMovePieces = 4096;  // 16-byte pieces a block copies at a time, about
 constexpr int kMaxMovesAtOnce = 128;
@@ -62,15 +64,14 @@ struct EvictParams {
 };
 
 struct EvictShared {
-    uint32_t hist[kBins];
+    uint32_t hist[kPasses][kBins];  // one for each pass: peers may still read one pass's counts while the next counts
     uint32_t warp_sum[kEvictWarps];
-    uint32_t prefix;   // digits found so far
-    uint32_t above;    // keys still to be kept within the prefix
-    uint32_t counts;   // this CTA's keys equal to the threshold
-    uint32_t holes;    // this CTA's holes
-    uint32_t movers;   // this CTA's movers
+    uint32_t prefix;  // bytes found so far
+    uint32_t wanted;  // keys still to be kept within the prefix
+    uint32_t equal;   // this CTA's keys equal to the threshold
+    uint32_t holes;   // this CTA's holes
+    uint32_t movers;  // this CTA's movers
     int32_t newest;
-    uint32_t total;
 };
 
 // Unsigned order of the result = order of the weights; both zeros are equal, NaN is the largest.
@@ -80,17 +81,11 @@ __device__ __forceinline__ uint32_t WeightKey(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive scan of one value per thread; every thread also gets the total.
-__device__ __forceinline__ uint32_t BlockExclusive(uint32_t value, EvictShared &sh, uint32_t *total) {
-    const uint32_t lane = LaneId(), warp = threadIdx.x >> 5;
-    uint32_t inclusive = value;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
-        if (lane >= d) inclusive += up;
-    }
+// Exclusive sum over the warps of a value that each warp's lanes agree on; every thread also gets the total.
+__device__ __forceinline__ uint32_t WarpsExclusive(uint32_t value, EvictShared &sh, uint32_t *total) {
+    const uint32_t warp = threadIdx.x >> 5;
     __syncthreads();
-    if (lane == 31) sh.warp_sum[warp] = inclusive;
+    if (LaneId() == 0) sh.warp_sum[warp] = value;
     __syncthreads();
     uint32_t before = 0, all = 0;
 #pragma unroll
@@ -100,20 +95,28 @@ __device__ __forceinline__ uint32_t BlockExclusive(uint32_t value, EvictShared &
         all += s;
     }
     *total = all;
-    return before + inclusive - value;
+    return before;
 }
 
-template <bool kCached>
-__global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const EvictParams p) {
-    extern __shared__ uint32_t keys[];
+template <bool kCluster, bool kCached>
+__global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __grid_constant__ EvictParams p) {
+    extern __shared__ uint32_t slots[];  // keys, then positions, of this CTA's slice
     __shared__ EvictShared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t n_ranks = cluster.num_blocks();
-    const uint32_t rank = cluster.block_rank();
+    const uint32_t n_ranks = kCluster ? cluster.num_blocks() : 1;
+    const uint32_t rank = kCluster ? cluster.block_rank() : 0;
+    auto sync_all = [&]() {
+        if (kCluster) {
+            cluster.sync();
+        } else {
+            __syncthreads();
+        }
+    };
+    auto peer = [&](uint32_t r) -> const EvictShared & { return kCluster ? *cluster.map_shared_rank(&sh, r) : sh; };
     const uint32_t unit = blockIdx.x / n_ranks;
     const uint32_t seq = unit / p.n_heads;
     const uint32_t head = unit - seq * p.n_heads;
-    const uint32_t tid = threadIdx.x, lane = LaneId();
+    const uint32_t tid = threadIdx.x, lane = LaneId(), warp = tid >> 5;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
     int32_t n = __ldg(p.lens + seq);
@@ -139,149 +142,210 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const Evict
         return;  // every CTA of the cluster leaves here
     }
 
-    // This CTA's slice of the slots; within it a thread owns `per` consecutive ones, an odd number so that a warp's
-    // reads of the key array spread over the banks.
-    const int32_t slice = (n + n_ranks - 1) / n_ranks;
-    const int32_t per = ((slice + kEvictThreads - 1) / kEvictThreads) | 1;
+    const int32_t slice = (n + n_ranks - 1) / n_ranks;  // of the slots; the last one's may be shorter
     const int32_t first = min(n, static_cast<int32_t>(rank) * slice);
     const int32_t count = min(n, first + slice) - first;
+    w_in += first;
+    pos_in += first;
+    uint32_t *keys = slots;
+    int32_t *ages = reinterpret_cast<int32_t *>(slots + slice);
 
-    // The largest position in use, over the cluster.
+    // Weights and positions into shared memory; the largest position in use, over the cluster.
+    for (uint32_t i = tid; i < kPasses * kBins; i += kEvictThreads) (&sh.hist[0][0])[i] = 0;
+    if (tid == 0) {
+        sh.newest = INT32_MIN;
+        sh.prefix = 0;
+        sh.wanted = static_cast<uint32_t>(k);
+    }
     int32_t newest = INT32_MIN;
-    for (int32_t i = tid; i < count; i += kEvictThreads) newest = max(newest, pos_in[first + i]);
+    for (int32_t i0 = tid; i0 < count; i0 += kLoads * kEvictThreads) {
+        float w[kLoads];
+        int32_t age[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int32_t i = i0 + j * kEvictThreads;
+            age[j] = INT32_MIN;
+            if (i < count) {
+                age[j] = pos_in[i];
+                if (kCached) w[j] = w_in[i];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int32_t i = i0 + j * kEvictThreads;
+            newest = max(newest, age[j]);
+            if (kCached && i < count) {
+                keys[i] = WeightKey(w[j]);
+                ages[i] = age[j];
+            }
+        }
+    }
     newest = __reduce_max_sync(0xffffffffu, newest);
-    if (tid == 0) sh.newest = INT32_MIN;
     __syncthreads();
     if (lane == 0) atomicMax(&sh.newest, newest);
-    cluster.sync();
-    newest = INT32_MIN;
-    for (uint32_t r = 0; r < n_ranks; ++r) newest = max(newest, cluster.map_shared_rank(&sh, r)->newest);
+    sync_all();
+    newest = sh.newest;
+    if (kCluster) {
+        for (uint32_t r = 0; r < n_ranks; ++r) newest = max(newest, peer(r).newest);
+    }
     const int64_t oldest_safe = static_cast<int64_t>(newest) - p.recent;  // protected: position > oldest_safe
 
-    auto make_key = [&](int32_t i) -> uint32_t {
-        return pos_in[first + i] > oldest_safe ? kKeyProtected : WeightKey(w_in[first + i]);
+    auto key_at = [&](int32_t i) -> uint32_t {
+        if (kCached) return keys[i];
+        return pos_in[i] > oldest_safe ? kKeyProtected : WeightKey(w_in[i]);
     };
-    auto key_at = [&](int32_t i) -> uint32_t { return kCached ? keys[i] : make_key(i); };
-    if (kCached) {
-        for (int32_t i = tid; i < count; i += kEvictThreads) keys[i] = make_key(i);
-    }
 
-    // The k-th largest key, digit by digit from the top.
-    if (tid == 0) {
-        sh.prefix = 0;
-        sh.above = static_cast<uint32_t>(k);
-    }
-    uint32_t mask = 0;  // bits of the key settled so far
+    // The k-th largest key, byte by byte from the top.
+    uint32_t prefix = 0, wanted = static_cast<uint32_t>(k);
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-        const uint32_t bins = pass == 2 ? 1024u : 2048u;
-        for (uint32_t b = tid; b < kBins; b += kEvictThreads) sh.hist[b] = 0;
-        __syncthreads();
-        const uint32_t prefix = sh.prefix;
-        for (int32_t i = tid; i < count; i += kEvictThreads) {
-            const uint32_t key = key_at(i);
-            if ((key & mask) == prefix) atomicAdd(&sh.hist[(key >> shift) & (bins - 1)], 1u);
-        }
-        cluster.sync();
-        // Thread t adds up bins 4t' .. of the whole cluster, from the top bin down.
-        constexpr int kPer = kBins / kEvictThreads;
-        uint32_t sums[kPer];
-        uint32_t mine = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const uint32_t bin = kBins - 1 - (tid * kPer + j);
-            sums[j] = 0;
-            for (uint32_t r = 0; r < n_ranks; ++r) sums[j] += cluster.map_shared_rank(&sh, r)->hist[bin];
-            mine += sums[j];
-        }
-        uint32_t total;
-        uint32_t before = BlockExclusive(mine, sh, &total);
-        const uint32_t wanted = sh.above;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const uint32_t bin = kBins - 1 - (tid * kPer + j);
-            if (before < wanted && before + sums[j] >= wanted) {
-                sh.prefix = prefix | (bin << shift);
-                sh.above = wanted - before;
-                sh.counts = sh.hist[bin];  // of this CTA
+    for (int pass = 0; pass < kPasses; ++pass) {
+        const int shift = 24 - 8 * pass;
+        const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
+        uint32_t *hist = sh.hist[pass];
+        for (int32_t i0 = warp * 32; i0 < count; i0 += kEvictThreads) {
+            const int32_t i = i0 + static_cast<int32_t>(lane);
+            uint32_t key = 0;
+            bool counts = i < count;
+            if (counts) {
+                key = key_at(i);
+                if (kCached && pass == 0 && ages[i] > oldest_safe) keys[i] = key = kKeyProtected;
+                counts = (key & mask) == prefix;
             }
-            before += sums[j];
+            // Weights share their high bytes: lanes with the same byte add their number once.
+            const uint32_t byte = counts ? (key >> shift) & 0xffu : 0x100u;
+            const uint32_t same = __match_any_sync(0xffffffffu, byte);
+            if (counts && lane == static_cast<uint32_t>(__ffs(same)) - 1) atomicAdd(&hist[byte], static_cast<uint32_t>(__popc(same)));
         }
-        mask |= (bins - 1) << shift;
-        cluster.sync();  // the counts are read by all before they are cleared
+        sync_all();
+        if (warp == 0) {
+            // Lane t takes the eight bytes 255 - 8 t .. 248 - 8 t, from the top down.
+            uint32_t sums[8] = {};
+            for (uint32_t r = 0; r < n_ranks; ++r) {
+                const uint4 *from = reinterpret_cast<const uint4 *>(&peer(r).hist[pass][248 - 8 * lane]);
+                const uint4 lo = from[0], hi = from[1];
+                sums[0] += hi.w;
+                sums[1] += hi.z;
+                sums[2] += hi.y;
+                sums[3] += hi.x;
+                sums[4] += lo.w;
+                sums[5] += lo.z;
+                sums[6] += lo.y;
+                sums[7] += lo.x;
+            }
+            uint32_t mine = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine += sums[j];
+            uint32_t inclusive = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
+                if (lane >= d) inclusive += up;
+            }
+            uint32_t before = inclusive - mine;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (before < wanted && before + sums[j] >= wanted) {
+                    const uint32_t byte = 255 - (8 * lane + j);
+                    sh.prefix = prefix | (byte << shift);
+                    sh.wanted = wanted - before;
+                    sh.equal = hist[byte];  // of this CTA; after the last pass, keys equal to the threshold
+                }
+                before += sums[j];
+            }
+        }
+        __syncthreads();
+        prefix = sh.prefix;
+        wanted = sh.wanted;
     }
-    const uint32_t threshold = sh.prefix;
-    const uint32_t equal_kept = sh.above;  // of the keys equal to the threshold, those in the lowest slots
+    const uint32_t threshold = prefix;
+    const uint32_t equal_kept = wanted;  // of the keys equal to the threshold, those in the lowest slots
+    sync_all();
 
-    // Which slots are holes and which are movers, in slot order.
-    uint32_t equal_base = 0;
-    for (uint32_t r = 0; r < rank; ++r) equal_base += cluster.map_shared_rank(&sh, r)->counts;
-    const int32_t begin = min(count, static_cast<int32_t>(tid) * per);
-    const int32_t end = min(count, begin + per);
-    uint32_t equal = 0;
-    for (int32_t i = begin; i < end; ++i) equal += key_at(i) == threshold;
-    uint32_t total;
-    const uint32_t equal_first = equal_base + BlockExclusive(equal, sh, &total);
-    uint32_t holes = 0, movers = 0, seen = equal_first;
-    for (int32_t i = begin; i < end; ++i) {
-        const uint32_t key = key_at(i);
-        const bool kept = key > threshold || (key == threshold && seen++ < equal_kept);
-        holes += !kept && first + i < k;
-        movers += kept && first + i >= k;
+    // Which slots are holes and which are movers, in slot order: each warp goes through a stretch of the slice, 32
+    // slots at a time.
+    uint32_t equal_before = 0;
+    if (kCluster) {
+        for (uint32_t r = 0; r < rank; ++r) equal_before += peer(r).equal;
+    }
+    const int32_t stretch = ((count + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
+    const int32_t begin = min(count, static_cast<int32_t>(warp) * stretch), end = min(count, begin + stretch);
+    const uint32_t below = (1u << lane) - 1u;
+    uint32_t total, equal = 0;
+    for (int32_t i0 = begin; i0 < end; i0 += 32) {
+        const int32_t i = i0 + static_cast<int32_t>(lane);
+        equal += __popc(__ballot_sync(0xffffffffu, i < end && key_at(i) == threshold));
+    }
+    equal_before += WarpsExclusive(equal, sh, &total);
+    // Whether the lane's slot is kept; `seen` counts the keys equal to the threshold so far.
+    auto is_kept = [&](int32_t i, uint32_t &seen) -> bool {
+        const uint32_t key = i < end ? key_at(i) : 0u;
+        const bool equals = i < end && key == threshold;
+        const uint32_t equals_mask = __ballot_sync(0xffffffffu, equals);
+        const bool kept = i < end && (key > threshold || (equals && seen + __popc(equals_mask & below) < equal_kept));
+        seen += __popc(equals_mask);
+        return kept;
+    };
+    uint32_t holes = 0, movers = 0, seen = equal_before;
+    for (int32_t i0 = begin; i0 < end; i0 += 32) {
+        const int32_t i = i0 + static_cast<int32_t>(lane), slot = first + i;
+        const bool kept = is_kept(i, seen);
+        holes += __popc(__ballot_sync(0xffffffffu, i < end && !kept && slot < k));
+        movers += __popc(__ballot_sync(0xffffffffu, kept && slot >= k));
     }
     uint32_t all_holes, all_movers;
-    uint32_t hole_at = BlockExclusive(holes, sh, &all_holes);
-    uint32_t mover_at = BlockExclusive(movers, sh, &all_movers);
+    uint32_t hole_at = WarpsExclusive(holes, sh, &all_holes);
+    uint32_t mover_at = WarpsExclusive(movers, sh, &all_movers);
     if (tid == 0) {
         sh.holes = all_holes;
         sh.movers = all_movers;
     }
-    cluster.sync();
-    uint32_t n_moves = 0;
-    for (uint32_t r = 0; r < n_ranks; ++r) {
-        const EvictShared *peer = cluster.map_shared_rank(&sh, r);
-        if (r < rank) {
-            hole_at += peer->holes;
-            mover_at += peer->movers;
+    uint32_t n_moves = all_movers;
+    if (kCluster) {
+        cluster.sync();
+        n_moves = 0;
+        for (uint32_t r = 0; r < n_ranks; ++r) {
+            if (r < rank) {
+                hole_at += peer(r).holes;
+                mover_at += peer(r).movers;
+            }
+            n_moves += peer(r).movers;
         }
-        n_moves += peer->movers;
+        cluster.sync();  // a CTA's shared memory may go once its peers have read it
     }
     if (rank == 0 && tid == 0) p.n_moves[unit] = static_cast<int32_t>(n_moves);
-    cluster.sync();  // a CTA's shared memory may go once its peers have read it
     int2 *moves = p.moves + static_cast<int64_t>(unit) * p.max_moves;
-    seen = equal_first;
-    for (int32_t i = begin; i < end; ++i) {
-        const uint32_t key = key_at(i);
-        const bool kept = key > threshold || (key == threshold && seen++ < equal_kept);
-        const int32_t slot = first + i;
-        if (slot < k) {
-            if (!kept) {
-                moves[hole_at++].y = slot;
-            } else if (p.separate_out) {
-                w_out[slot] = w_in[slot];
-                pos_out[slot] = pos_in[slot];
-            }
-        } else if (kept) {
-            moves[mover_at++].x = slot;
-        } else {
+    seen = equal_before;
+    for (int32_t i0 = begin; i0 < end; i0 += 32) {
+        const int32_t i = i0 + static_cast<int32_t>(lane), slot = first + i;
+        const bool kept = is_kept(i, seen);
+        const bool hole = i < end && !kept && slot < k, mover = kept && slot >= k;
+        const uint32_t hole_mask = __ballot_sync(0xffffffffu, hole), mover_mask = __ballot_sync(0xffffffffu, mover);
+        if (hole) moves[hole_at + __popc(hole_mask & below)].y = slot;
+        if (mover) moves[mover_at + __popc(mover_mask & below)].x = slot;
+        hole_at += __popc(hole_mask);
+        mover_at += __popc(mover_mask);
+        if (i < end && !kept && slot >= k) {
             w_out[slot] = 0.0f;
             pos_out[slot] = -1;
+        } else if (p.separate_out && kept && slot < k) {
+            w_out[slot] = w_in[i];
+            pos_out[slot] = pos_in[i];
         }
     }
 }
 
 // The moves: rows of K and V in 16-byte pieces, weight and position; the slot a token leaves becomes free.
-__global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_constant__ EvictParams p) {
     __shared__ int64_t from_row[kMaxMovesAtOnce], to_row[kMaxMovesAtOnce];
     const uint32_t tid = threadIdx.x;
     const uint32_t pieces = 2u * p.chunks * p.heads_per_move;  // of one move: K and V rows of every head that moves
     const int64_t blocks = static_cast<int64_t>(p.units) * p.blocks_per_unit;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-        const int32_t unit = static_cast<int32_t>(block / p.blocks_per_unit);
-        const int32_t at = static_cast<int32_t>(block - static_cast<int64_t>(unit) * p.blocks_per_unit) * p.moves_at_once;
+        // the first moves of every head, then the second ones: heads with fewer moves than there is room for run out last
+        const int64_t turn = block / p.units;
+        const int32_t unit = static_cast<int32_t>(block - turn * p.units);
+        const int32_t at = static_cast<int32_t>(turn) * p.moves_at_once;
         const int32_t here = min(p.moves_at_once, __ldcg(p.n_moves + unit) - at);
         if (here <= 0) continue;
         const int32_t seq = unit / p.n_heads, head = unit - seq * p.n_heads;
@@ -434,9 +498,9 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     const int32_t sm_count = GetDeviceInfo().sm_count;
     int cluster = 1;
     while (cluster < kMaxCluster && units * cluster * 2 <= 2 * sm_count && table_tokens / (cluster * 2) >= 1024) cluster *= 2;
-    while (cluster < kMaxCluster && (table_tokens + cluster - 1) / cluster > kMaxCachedKeys) cluster *= 2;
+    while (cluster < kMaxCluster && (table_tokens + cluster - 1) / cluster > kMaxCachedSlots) cluster *= 2;
     const int64_t slice = (table_tokens + cluster - 1) / cluster;
-    const bool cached = slice <= kMaxCachedKeys;
+    const bool cached = slice <= kMaxCachedSlots;
     p.units = static_cast<int32_t>(units);
     p.n_moves = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(d_workspace) + EvictMovesBytes(units, table_tokens, budget));
     const int32_t pieces = 2 * p.chunks * p.heads_per_move;
@@ -446,7 +510,7 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<uint32_t>(units * cluster));
     cfg.blockDim = dim3(kEvictThreads);
-    cfg.dynamicSmemBytes = cached ? static_cast<size_t>(slice) * 4 : 0;
+    cfg.dynamicSmemBytes = cached ? static_cast<size_t>(slice) * 8 : 0;
     cfg.stream = AsStream(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -454,12 +518,15 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cached) {
-        EnsureDynamicSmem(EvictPagesKernel<true>, kMaxCachedKeys * 4);
-        cudaLaunchKernelEx(&cfg, EvictPagesKernel<true>, p);
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    auto launch = [&](auto kernel) {
+        if (cached) EnsureDynamicSmem(kernel, kMaxCachedSlots * 8);
+        cudaLaunchKernelEx(&cfg, kernel, p);
+    };
+    if (cluster > 1) {
+        cached ? launch(EvictPagesKernel<true, true>) : launch(EvictPagesKernel<true, false>);
     } else {
-        cudaLaunchKernelEx(&cfg, EvictPagesKernel<false>, p);
+        launch(EvictPagesKernel<false, true>);  // a slice too long for shared memory has made a cluster above
     }
     if (p.blocks_per_unit == 0) return LaunchStatus();  // the budget is not below what the table holds
     cudaLaunchConfig_t move = {};
