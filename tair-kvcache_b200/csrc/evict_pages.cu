@@ -26,9 +26,11 @@ constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 256;
 constexpr int kPasses = 4;
+constexpr int kCopies = 4;  // of the counts, for lanes that count the same byte: weights share their high ones
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kKeyProtected = 0xFFFFFFFFu;
 constexpr uint32_t kKeyNan = 0xFFFFFFFEu;
+constexpr uint32_t kAll = 0xFFFFFFFFu;
 // Slots a CTA keeps in shared memory, key and position; longer slices are read again from global memory in every pass.
 constexpr int kMaxCachedSlots = 24576;
 constexpr int kLoads = 8;  // loads of a thread in flight together
@@ -64,8 +66,8 @@ struct EvictParams {
 };
 
 struct EvictShared {
-    uint32_t hist[kPasses][kBins];  // one for each pass: peers may still read one pass's counts while the next counts
-    uint32_t warp_sum[kEvictWarps];
+    uint32_t hist[kPasses][kCopies][kBins + 8];  // one for each pass: peers may still read one pass's while the next counts
+    uint2 warp_sum[kEvictWarps];
     uint32_t prefix;  // bytes found so far
     uint32_t wanted;  // keys still to be kept within the prefix
     uint32_t equal;   // this CTA's keys equal to the threshold
@@ -81,18 +83,22 @@ __device__ __forceinline__ uint32_t WeightKey(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive sum over the warps of a value that each warp's lanes agree on; every thread also gets the total.
-__device__ __forceinline__ uint32_t WarpsExclusive(uint32_t value, EvictShared &sh, uint32_t *total) {
+// Exclusive sums over the warps of two values that each warp's lanes agree on; every thread also gets the totals.
+__device__ __forceinline__ uint2 WarpsExclusive(uint2 value, EvictShared &sh, uint2 *total) {
     const uint32_t warp = threadIdx.x >> 5;
     __syncthreads();
     if (LaneId() == 0) sh.warp_sum[warp] = value;
     __syncthreads();
-    uint32_t before = 0, all = 0;
+    uint2 before = make_uint2(0, 0), all = make_uint2(0, 0);
 #pragma unroll
     for (int w = 0; w < kEvictWarps; ++w) {
-        const uint32_t s = sh.warp_sum[w];
-        if (w < static_cast<int>(warp)) before += s;
-        all += s;
+        const uint2 s = sh.warp_sum[w];
+        if (w < static_cast<int>(warp)) {
+            before.x += s.x;
+            before.y += s.y;
+        }
+        all.x += s.x;
+        all.y += s.y;
     }
     *total = all;
     return before;
@@ -100,7 +106,7 @@ __device__ __forceinline__ uint32_t WarpsExclusive(uint32_t value, EvictShared &
 
 template <bool kCluster, bool kCached>
 __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __grid_constant__ EvictParams p) {
-    extern __shared__ uint32_t slots[];  // keys, then positions, of this CTA's slice
+    extern __shared__ uint32_t slots[];  // weights, then positions, of this CTA's slice
     __shared__ EvictShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t n_ranks = kCluster ? cluster.num_blocks() : 1;
@@ -147,11 +153,11 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     const int32_t count = min(n, first + slice) - first;
     w_in += first;
     pos_in += first;
-    uint32_t *keys = slots;
+    float *held = reinterpret_cast<float *>(slots);
     int32_t *ages = reinterpret_cast<int32_t *>(slots + slice);
 
     // Weights and positions into shared memory; the largest position in use, over the cluster.
-    for (uint32_t i = tid; i < kPasses * kBins; i += kEvictThreads) (&sh.hist[0][0])[i] = 0;
+    for (uint32_t i = tid; i < sizeof(sh.hist) / 4; i += kEvictThreads) (&sh.hist[0][0][0])[i] = 0;
     if (tid == 0) {
         sh.newest = INT32_MIN;
         sh.prefix = 0;
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             const int32_t i = i0 + j * kEvictThreads;
             newest = max(newest, age[j]);
             if (kCached && i < count) {
-                keys[i] = WeightKey(w[j]);
+                held[i] = w[j];
                 ages[i] = age[j];
             }
         }
@@ -191,8 +197,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     const int64_t oldest_safe = static_cast<int64_t>(newest) - p.recent;  // protected: position > oldest_safe
 
     auto key_at = [&](int32_t i) -> uint32_t {
-        if (kCached) return keys[i];
-        return pos_in[i] > oldest_safe ? kKeyProtected : WeightKey(w_in[i]);
+        return (kCached ? ages[i] : pos_in[i]) > oldest_safe ? kKeyProtected : WeightKey(kCached ? held[i] : w_in[i]);
     };
 
     // The k-th largest key, byte by byte from the top.
@@ -201,36 +206,30 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     for (int pass = 0; pass < kPasses; ++pass) {
         const int shift = 24 - 8 * pass;
         const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
-        uint32_t *hist = sh.hist[pass];
-        for (int32_t i0 = warp * 32; i0 < count; i0 += kEvictThreads) {
-            const int32_t i = i0 + static_cast<int32_t>(lane);
-            uint32_t key = 0;
-            bool counts = i < count;
-            if (counts) {
-                key = key_at(i);
-                if (kCached && pass == 0 && ages[i] > oldest_safe) keys[i] = key = kKeyProtected;
-                counts = (key & mask) == prefix;
-            }
-            // Weights share their high bytes: lanes with the same byte add their number once.
-            const uint32_t byte = counts ? (key >> shift) & 0xffu : 0x100u;
-            const uint32_t same = __match_any_sync(0xffffffffu, byte);
-            if (counts && lane == static_cast<uint32_t>(__ffs(same)) - 1) atomicAdd(&hist[byte], static_cast<uint32_t>(__popc(same)));
+        uint32_t *hist = sh.hist[pass][lane % kCopies];
+#pragma unroll 4
+        for (int32_t i = tid; i < count; i += kEvictThreads) {
+            const uint32_t key = key_at(i);
+            if ((key & mask) == prefix) atomicAdd(hist + ((key >> shift) & 0xffu), 1u);
         }
         sync_all();
         if (warp == 0) {
             // Lane t takes the eight bytes 255 - 8 t .. 248 - 8 t, from the top down.
             uint32_t sums[8] = {};
             for (uint32_t r = 0; r < n_ranks; ++r) {
-                const uint4 *from = reinterpret_cast<const uint4 *>(&peer(r).hist[pass][248 - 8 * lane]);
-                const uint4 lo = from[0], hi = from[1];
-                sums[0] += hi.w;
-                sums[1] += hi.z;
-                sums[2] += hi.y;
-                sums[3] += hi.x;
-                sums[4] += lo.w;
-                sums[5] += lo.z;
-                sums[6] += lo.y;
-                sums[7] += lo.x;
+#pragma unroll
+                for (int c = 0; c < kCopies; ++c) {
+                    const uint4 *from = reinterpret_cast<const uint4 *>(&peer(r).hist[pass][c][248 - 8 * lane]);
+                    const uint4 lo = from[0], hi = from[1];
+                    sums[0] += hi.w;
+                    sums[1] += hi.z;
+                    sums[2] += hi.y;
+                    sums[3] += hi.x;
+                    sums[4] += lo.w;
+                    sums[5] += lo.z;
+                    sums[6] += lo.y;
+                    sums[7] += lo.x;
+                }
             }
             uint32_t mine = 0;
 #pragma unroll
@@ -247,8 +246,11 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
                 if (before < wanted && before + sums[j] >= wanted) {
                     const uint32_t byte = 255 - (8 * lane + j);
                     sh.prefix = prefix | (byte << shift);
-                    sh.wanted = wanted - before;
-                    sh.equal = hist[byte];  // of this CTA; after the last pass, keys equal to the threshold
+                    sh.wanted = before + sums[j] == wanted ? kAll : wanted - before;
+                    uint32_t own = 0;  // after the last pass, keys of this CTA that are equal to the threshold
+#pragma unroll
+                    for (int c = 0; c < kCopies; ++c) own += sh.hist[pass][c][byte];
+                    sh.equal = own;
                 }
                 before += sums[j];
             }
@@ -256,29 +258,35 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
         __syncthreads();
         prefix = sh.prefix;
         wanted = sh.wanted;
+        if (wanted == kAll) break;  // every key that begins with these bytes is kept: nothing is left to tell apart
     }
     const uint32_t threshold = prefix;
     const uint32_t equal_kept = wanted;  // of the keys equal to the threshold, those in the lowest slots
-    sync_all();
+    const bool ties = wanted != kAll;
 
     // Which slots are holes and which are movers, in slot order: each warp goes through a stretch of the slice, 32
     // slots at a time.
-    uint32_t equal_before = 0;
-    if (kCluster) {
-        for (uint32_t r = 0; r < rank; ++r) equal_before += peer(r).equal;
-    }
     const int32_t stretch = ((count + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
     const int32_t begin = min(count, static_cast<int32_t>(warp) * stretch), end = min(count, begin + stretch);
     const uint32_t below = (1u << lane) - 1u;
-    uint32_t total, equal = 0;
-    for (int32_t i0 = begin; i0 < end; i0 += 32) {
-        const int32_t i = i0 + static_cast<int32_t>(lane);
-        equal += __popc(__ballot_sync(0xffffffffu, i < end && key_at(i) == threshold));
+    uint32_t equal_before = 0;
+    if (ties) {
+        sync_all();
+        if (kCluster) {
+            for (uint32_t r = 0; r != rank; ++r) equal_before += peer(r).equal;
+        }
+        uint32_t equal = 0;
+        for (int32_t i0 = begin; i0 < end; i0 += 32) {
+            const int32_t i = i0 + static_cast<int32_t>(lane);
+            equal += __popc(__ballot_sync(0xffffffffu, i < end && key_at(i) == threshold));
+        }
+        uint2 total;
+        equal_before += WarpsExclusive(make_uint2(equal, 0), sh, &total).x;
     }
-    equal_before += WarpsExclusive(equal, sh, &total);
     // Whether the lane's slot is kept; `seen` counts the keys equal to the threshold so far.
     auto is_kept = [&](int32_t i, uint32_t &seen) -> bool {
         const uint32_t key = i < end ? key_at(i) : 0u;
+        if (!ties) return i < end && key >= threshold;
         const bool equals = i < end && key == threshold;
         const uint32_t equals_mask = __ballot_sync(0xffffffffu, equals);
         const bool kept = i < end && (key > threshold || (equals && seen + __popc(equals_mask & below) < equal_kept));
@@ -292,19 +300,19 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
         holes += __popc(__ballot_sync(0xffffffffu, i < end && !kept && slot < k));
         movers += __popc(__ballot_sync(0xffffffffu, kept && slot >= k));
     }
-    uint32_t all_holes, all_movers;
-    uint32_t hole_at = WarpsExclusive(holes, sh, &all_holes);
-    uint32_t mover_at = WarpsExclusive(movers, sh, &all_movers);
+    uint2 all;
+    const uint2 mine_at = WarpsExclusive(make_uint2(holes, movers), sh, &all);
+    uint32_t hole_at = mine_at.x, mover_at = mine_at.y;
     if (tid == 0) {
-        sh.holes = all_holes;
-        sh.movers = all_movers;
+        sh.holes = all.x;
+        sh.movers = all.y;
     }
-    uint32_t n_moves = all_movers;
+    uint32_t n_moves = all.y;
     if (kCluster) {
         cluster.sync();
         n_moves = 0;
         for (uint32_t r = 0; r < n_ranks; ++r) {
-            if (r < rank) {
+            if (kCluster && r < rank) {
                 hole_at += peer(r).holes;
                 mover_at += peer(r).movers;
             }
@@ -328,8 +336,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             w_out[slot] = 0.0f;
             pos_out[slot] = -1;
         } else if (p.separate_out && kept && slot < k) {
-            w_out[slot] = w_in[i];
-            pos_out[slot] = pos_in[i];
+            w_out[slot] = kCached ? held[i] : w_in[i];
+            pos_out[slot] = kCached ? ages[i] : pos_in[i];
         }
     }
 }
