@@ -27,12 +27,12 @@ constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 256;
 constexpr int kPasses = 4;
 constexpr int kCopies = 4;  // of the counts, for lanes that count the same byte: weights share their high ones
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;  // beyond 8 a launch opts in
 constexpr uint32_t kKeyProtected = 0xFFFFFFFFu;
 constexpr uint32_t kKeyNan = 0xFFFFFFFEu;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 // Slots a CTA keeps in shared memory, key and position; longer slices are read again from global memory in every pass.
-constexpr int kMaxCachedSlots = 24576;
+constexpr int kMaxCachedSlots = 22528;
 constexpr int kLoads = 8;  // loads of a thread in flight together
 constexpr int kMoveThreads = 256;
 constexpr int kMovePieces = 4096;  // 16-byte pieces a block copies at a time, about
@@ -65,7 +65,9 @@ struct EvictParams {
     int32_t blocks_per_unit;
 };
 
+template <bool kCluster>
 struct EvictShared {
+    uint32_t merged[kCluster ? kMaxCluster : 1][kBins];  // a pass's counts of every CTA of the cluster
     uint32_t hist[kPasses][kCopies][kBins + 8];  // one for each pass: peers may still read one pass's while the next counts
     uint2 warp_sum[kEvictWarps];
     uint32_t prefix;  // bytes found so far
@@ -84,7 +86,8 @@ __device__ __forceinline__ uint32_t WeightKey(float w) {
 }
 
 // Exclusive sums over the warps of two values that each warp's lanes agree on; every thread also gets the totals.
-__device__ __forceinline__ uint2 WarpsExclusive(uint2 value, EvictShared &sh, uint2 *total) {
+template <bool kCluster>
+__device__ __forceinline__ uint2 WarpsExclusive(uint2 value, EvictShared<kCluster> &sh, uint2 *total) {
     const uint32_t warp = threadIdx.x >> 5;
     __syncthreads();
     if (LaneId() == 0) sh.warp_sum[warp] = value;
@@ -106,8 +109,8 @@ __device__ __forceinline__ uint2 WarpsExclusive(uint2 value, EvictShared &sh, ui
 
 template <bool kCluster, bool kCached>
 __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __grid_constant__ EvictParams p) {
-    extern __shared__ uint32_t slots[];  // weights, then positions, of this CTA's slice
-    __shared__ EvictShared sh;
+    extern __shared__ uint32_t slots[];  // keys, then positions, of this CTA's slice
+    __shared__ EvictShared<kCluster> sh;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t n_ranks = kCluster ? cluster.num_blocks() : 1;
     const uint32_t rank = kCluster ? cluster.block_rank() : 0;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             __syncthreads();
         }
     };
-    auto peer = [&](uint32_t r) -> const EvictShared & { return kCluster ? *cluster.map_shared_rank(&sh, r) : sh; };
+    auto peer = [&](uint32_t r) -> const EvictShared<kCluster> & { return kCluster ? *cluster.map_shared_rank(&sh, r) : sh; };
     const uint32_t unit = blockIdx.x / n_ranks;
     const uint32_t seq = unit / p.n_heads;
     const uint32_t head = unit - seq * p.n_heads;
@@ -153,8 +156,9 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     const int32_t count = min(n, first + slice) - first;
     w_in += first;
     pos_in += first;
-    float *held = reinterpret_cast<float *>(slots);
+    uint32_t *keys = slots;
     int32_t *ages = reinterpret_cast<int32_t *>(slots + slice);
+    uint32_t *kept_bits = slots + slice;  // in the place of the positions, once the keys account for them
 
     // Weights and positions into shared memory; the largest position in use, over the cluster.
     for (uint32_t i = tid; i < sizeof(sh.hist) / 4; i += kEvictThreads) (&sh.hist[0][0][0])[i] = 0;
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             const int32_t i = i0 + j * kEvictThreads;
             newest = max(newest, age[j]);
             if (kCached && i < count) {
-                held[i] = w[j];
+                keys[i] = WeightKey(w[j]);
                 ages[i] = age[j];
             }
         }
@@ -197,7 +201,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     const int64_t oldest_safe = static_cast<int64_t>(newest) - p.recent;  // protected: position > oldest_safe
 
     auto key_at = [&](int32_t i) -> uint32_t {
-        return (kCached ? ages[i] : pos_in[i]) > oldest_safe ? kKeyProtected : WeightKey(kCached ? held[i] : w_in[i]);
+        if (kCached) return keys[i];
+        return pos_in[i] > oldest_safe ? kKeyProtected : WeightKey(w_in[i]);
     };
 
     // The k-th largest key, byte by byte from the top.
@@ -209,28 +214,44 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
         uint32_t *hist = sh.hist[pass][lane % kCopies];
 #pragma unroll 4
         for (int32_t i = tid; i < count; i += kEvictThreads) {
-            const uint32_t key = key_at(i);
+            uint32_t key = key_at(i);
+            if (kCached && pass == 0 && ages[i] > oldest_safe) keys[i] = key = kKeyProtected;
             if ((key & mask) == prefix) atomicAdd(hist + ((key >> shift) & 0xffu), 1u);
         }
         sync_all();
-        if (warp == 0) {
-            // Lane t takes the eight bytes 255 - 8 t .. 248 - 8 t, from the top down.
-            uint32_t sums[8] = {};
-            for (uint32_t r = 0; r < n_ranks; ++r) {
+        // Lane t takes the eight bytes 255 - 8 t .. 248 - 8 t, from the top down; the copies of a CTA's counts are added up
+        // by a warp, those of a cluster by a warp each.
+        uint32_t sums[8] = {};
+        if (warp < n_ranks) {
 #pragma unroll
-                for (int c = 0; c < kCopies; ++c) {
-                    const uint4 *from = reinterpret_cast<const uint4 *>(&peer(r).hist[pass][c][248 - 8 * lane]);
-                    const uint4 lo = from[0], hi = from[1];
-                    sums[0] += hi.w;
-                    sums[1] += hi.z;
-                    sums[2] += hi.y;
-                    sums[3] += hi.x;
-                    sums[4] += lo.w;
-                    sums[5] += lo.z;
-                    sums[6] += lo.y;
-                    sums[7] += lo.x;
+            for (int c = 0; c < kCopies; ++c) {
+                const uint4 *from = reinterpret_cast<const uint4 *>(&peer(warp).hist[pass][c][248 - 8 * lane]);
+                const uint4 lo = from[0], hi = from[1];
+                sums[0] += hi.w;
+                sums[1] += hi.z;
+                sums[2] += hi.y;
+                sums[3] += hi.x;
+                sums[4] += lo.w;
+                sums[5] += lo.z;
+                sums[6] += lo.y;
+                sums[7] += lo.x;
+            }
+        }
+        if (kCluster) {
+            if (warp < n_ranks) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sh.merged[warp][j * 32 + lane] = sums[j];
+            }
+            __syncthreads();
+            if (warp == 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sums[j] = 0;
+                    for (uint32_t r = 0; r < n_ranks; ++r) sums[j] += sh.merged[r][j * 32 + lane];
                 }
             }
+        }
+        if (warp == 0) {
             uint32_t mine = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) mine += sums[j];
@@ -297,8 +318,11 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     for (int32_t i0 = begin; i0 < end; i0 += 32) {
         const int32_t i = i0 + static_cast<int32_t>(lane), slot = first + i;
         const bool kept = is_kept(i, seen);
-        holes += __popc(__ballot_sync(0xffffffffu, i < end && !kept && slot < k));
-        movers += __popc(__ballot_sync(0xffffffffu, kept && slot >= k));
+        const uint32_t kept_mask = __ballot_sync(0xffffffffu, kept);
+        const uint32_t low_mask = __ballot_sync(0xffffffffu, i < end && slot < k);
+        holes += __popc(low_mask & ~kept_mask);
+        movers += __popc(kept_mask & ~low_mask);
+        if (kCached && lane == 0) kept_bits[i0 >> 5] = kept_mask;
     }
     uint2 all;
     const uint2 mine_at = WarpsExclusive(make_uint2(holes, movers), sh, &all);
@@ -325,7 +349,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
     seen = equal_before;
     for (int32_t i0 = begin; i0 < end; i0 += 32) {
         const int32_t i = i0 + static_cast<int32_t>(lane), slot = first + i;
-        const bool kept = is_kept(i, seen);
+        const bool kept = kCached ? (kept_bits[i0 >> 5] >> lane) & 1u : is_kept(i, seen);
         const bool hole = i < end && !kept && slot < k, mover = kept && slot >= k;
         const uint32_t hole_mask = __ballot_sync(0xffffffffu, hole), mover_mask = __ballot_sync(0xffffffffu, mover);
         if (hole) moves[hole_at + __popc(hole_mask & below)].y = slot;
@@ -335,9 +359,33 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
         if (i < end && !kept && slot >= k) {
             w_out[slot] = 0.0f;
             pos_out[slot] = -1;
-        } else if (p.separate_out && kept && slot < k) {
-            w_out[slot] = kCached ? held[i] : w_in[i];
-            pos_out[slot] = kCached ? ages[i] : pos_in[i];
+        } else if (!kCached && p.separate_out && kept && slot < k) {
+            w_out[slot] = w_in[i];
+            pos_out[slot] = pos_in[i];
+        }
+    }
+    if (kCached && p.separate_out) {  // survivors that stay
+        __syncthreads();
+        const int32_t low = min(count, k - first);
+        for (int32_t i0 = tid; i0 < low; i0 += kLoads * kEvictThreads) {
+            float w[kLoads];
+            int32_t age[kLoads];
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int32_t i = i0 + j * kEvictThreads;
+                if (i < low && ((kept_bits[i >> 5] >> (i & 31)) & 1u)) {
+                    w[j] = w_in[i];
+                    age[j] = pos_in[i];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int32_t i = i0 + j * kEvictThreads;
+                if (i < low && ((kept_bits[i >> 5] >> (i & 31)) & 1u)) {
+                    w_out[first + i] = w[j];
+                    pos_out[first + i] = age[j];
+                }
+            }
         }
     }
 }
@@ -385,7 +433,7 @@ __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_con
         }
         __syncthreads();
         const uint32_t n_pieces = static_cast<uint32_t>(here) * pieces;
-        constexpr int kUnroll = 4;
+        constexpr int kUnroll = 8;
         for (uint32_t base = tid; base < n_pieces; base += kMoveThreads * kUnroll) {
             uint4 data[kUnroll];
             uint8_t *to[kUnroll];
@@ -412,6 +460,12 @@ __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_con
             }
         }
     }
+}
+
+// The opt-in to clusters of more than eight CTAs is per device and per kernel, like the one to large shared memory.
+template <typename Kernel>
+void AllowLargeClusters(Kernel kernel) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 
 int64_t EvictMaxMoves(int64_t table_tokens, int32_t budget) {
@@ -529,6 +583,7 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     cfg.numAttrs = cluster > 1 ? 1 : 0;
     auto launch = [&](auto kernel) {
         if (cached) EnsureDynamicSmem(kernel, kMaxCachedSlots * 8);
+        if (cluster > 8) AllowLargeClusters(kernel);
         cudaLaunchKernelEx(&cfg, kernel, p);
     };
     if (cluster > 1) {
