@@ -22,6 +22,7 @@
 // batch are numbered through, and each of the persistent CTAs takes an equal run of them, found from the lengths on the
 // device.  A head that lies within one run is finished there; the runs of a head that is cut leave their unnormalised
 // sums and statistics in the workspace, and the second kernel joins them, in order, so results do not depend on timing.
+// A third adds up the weights, which need every head's final statistics.
 #include "paged_kv.cuh"
 
 namespace kvcm {
@@ -54,7 +55,7 @@ struct AttendParams {
     // workspace
     float *part_o;          // [workers * 2][step_heads][rows][dim]
     float2 *part_ml;        // [workers * 2][step_heads][rows] maximum and sum of a share, the maximum in units of log2
-    float2 *whole_ml;       // [batch][n_q_heads], heads that one CTA finished
+    float2 *whole_ml;       // [batch][n_q_heads] maximum and sum of whole heads; with weights only
     float *scores;          // [batch][n_q_heads][score_stride], in units of log2; null without weights
     int64_t score_stride;
     int32_t batch, n_q_heads, group;
@@ -162,8 +163,15 @@ __device__ __forceinline__ float Log2(float x) {
     return y;
 }
 // 16 bytes, of which the first `bytes` come from src and the rest are zeros.
-__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void *src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// K and V rows are read once: they may leave L2 before what the kernels after this one read.
+__device__ __forceinline__ uint64_t ReadOncePolicy() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void *src, uint32_t bytes, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;\n" ::"r"(dst), "l"(src), "r"(bytes), "l"(policy)
+                 : "memory");
 }
 __device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int kPending>
@@ -330,6 +338,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
     const int64_t copy_from = static_cast<int64_t>(copy_row) * p.pools.token_stride + (copy_bytes != 0 ? copy_piece * 16 : 0);
     const int64_t copy_stride = kCopyRows * p.pools.token_stride;
     const int64_t v_minus_k = p.pools.v - p.pools.k;
+    const uint64_t policy = ReadOncePolicy();
     // Starts the copies of this warp's tile of the next step; rows that take no part become zeros, so that whatever lies
     // there cannot reach a product.
     auto load_tile = [&](int to_stage) {
@@ -349,8 +358,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
                     const uint32_t row = i * kCopyRows + copy_row;
                     const uint32_t bytes = (valid >> row) & 1u ? copy_bytes : 0u;
                     const uint32_t at = (to ^ (((i * kCopyRows) & 7) * 16)) + i * kCopyRows * Shape::kRowBytes;
-                    CopyAsync16(at, from, bytes);
-                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes);
+                    CopyAsync16(at, from, bytes, policy);
+                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes, policy);
                     from += copy_stride;
                 }
             }
@@ -365,8 +374,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
                     const uint32_t bytes = (valid >> row) & 1u ? copy_bytes : 0u;
                     const uint8_t *from = p.pools.k + (bytes != 0 ? row_off + copy_piece * 16 : 0);
                     const uint32_t at = (to ^ (((i * kCopyRows) & 7) * 16)) + i * kCopyRows * Shape::kRowBytes;
-                    CopyAsync16(at, from, bytes);
-                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes);
+                    CopyAsync16(at, from, bytes, policy);
+                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes, policy);
                 }
             }
         }
@@ -667,228 +676,168 @@ struct Partial {
     }
 };
 
-// Running maximum and sum over shares [from, to] of a head, every `by`-th.
-__device__ __forceinline__ float2 StatsOf(const AttendParams &p, const Shares &sh, int32_t kv_i, int32_t row, int32_t rows,
-                                          int32_t from, int32_t by) {
-    float m = -INFINITY, l = 0.0f;
-    for (int32_t w = from; w <= sh.last; w += by) {
-        const float2 ml = __ldcg(p.part_ml + (sh.Slot(w) * p.step_heads + kv_i) * rows + row);
-        const float grown = fmaxf(m, ml.x);
-        const float use = grown == -INFINITY ? 0.0f : grown;
-        l = l * Exp2(m - use) + ml.y * Exp2(ml.x - use);
-        m = grown;
-    }
-    return make_float2(m, l);
-}
-
-// Joins the shares of heads that were cut and, in the blocks behind those, adds the attention every token received to its
-// weight.  It starts when the first kernel's last CTA ends, so what counts is the chain of dependent loads after that:
-// small blocks, all resident at once, find their work from the lengths while the first kernel still runs, and load all
-// they need of its results together.
-//
-// Join: block w looks at the point where run w begins.  When that lies within a unit, the unit's shares are joined by
-// the blocks of all such points together: with c cuts each block takes a c-th of the unit's output elements, four to a
-// thread group, over all shares, so that one long head is joined by as many blocks as computed it.
-//
-// Weights: the steps of all sequences and weight heads are cut into equal runs again.
+// Joins the shares of heads that were cut.  It starts when the first kernel's last CTA ends, so what counts is the chain of
+// dependent loads after that: small blocks, all resident at once, find their work from the lengths while the first
+// kernel still runs, and load all they need of its results together.  Block w looks at the point where run w begins.
+// When that lies within a unit, the unit's shares are joined by the blocks of all such points together: with c cuts
+// each block takes a c-th of the unit's output elements, four to a thread group, over all shares, so that one long head
+// is joined by as many blocks as computed it.
 template <typename T, int kDim, int kRows, bool kScores>
-__global__ void __launch_bounds__(kJoinThreads, 8) JoinSharesKernel(const __grid_constant__ AttendParams p, int32_t weight_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 8) JoinSharesKernel(const __grid_constant__ AttendParams p) {
     __shared__ Partial partials[kJoinThreads / 32];
     __shared__ int64_t scan_warp[kJoinThreads / 32];
     __shared__ Place64 found;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const StepScan scan = ScanSteps<kJoinThreads>(p, scan_warp);
     const int64_t per = StepsPerRun(scan.all * p.units, p.workers);
-    if (blockIdx.x < static_cast<uint32_t>(p.workers)) {
-        const int32_t w = blockIdx.x;
-        if (w * per >= scan.all * p.units) return;
-        FindStep(p, scan, p.units, w * per, &found);
-        const int32_t b = found.b;
-        const int32_t steps = SpanOf(p, b).steps;
-        const int64_t inside = w * per - found.before;
-        const int32_t unit = static_cast<int32_t>(Divide(inside, steps));
-        const int64_t into = inside - static_cast<int64_t>(unit) * steps;
-        if (into == 0) return;  // nothing is cut here
-        const Shares sh = SharesAt(w * per - into, steps, per);
-        const int32_t cuts = sh.last - sh.first, cut = w - sh.first - 1;
-        const int32_t kvg = unit / p.row_tiles, row_tile = unit - kvg * p.row_tiles;
-        const int32_t rows = min(kRows, p.group - row_tile * kRows);
-        const int64_t head0 = static_cast<int64_t>(b) * p.n_q_heads + kvg * p.step_heads * p.group + row_tile * kRows;
-        const int32_t fours = p.step_heads * rows * (kDim / 4);    // groups of four output elements
-        const int32_t mine = (fours + cuts - 1) / cuts;            // this block's
-        int32_t lanes = 1;                                         // thread groups per pass, a power of two
-        while (lanes < mine && lanes < kJoinThreads) lanes *= 2;
-        const int32_t parts = kJoinThreads / lanes;                // threads that share a group's shares
-        const int32_t at = tid / parts, part = tid % parts;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int32_t w = blockIdx.x;
+    // Every block waits for the first kernel, also one without work: the kernel after this one relies on it.
+    if (w * per >= scan.all * p.units) {
         asm volatile("griddepcontrol.wait;\n" ::: "memory");
-        for (int32_t base = 0; base < mine; base += lanes) {
-            const int32_t four = cut * mine + base + at;
-            const bool live = base + at < mine && four < fours;
-            const int32_t head_row = live ? four / (kDim / 4) : 0, d = live ? (four - head_row * (kDim / 4)) * 4 : 0;
-            const int32_t kv_i = head_row / rows, row = head_row - kv_i * rows;
-            const int64_t head_at = head0 + kv_i * p.group + row;
-            Partial acc = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-            constexpr int kTogether = 4;
-            for (int32_t i0 = sh.first + part; live && i0 <= sh.last; i0 += kTogether * parts) {
-                Partial got[kTogether];
-#pragma unroll
-                for (int j = 0; j < kTogether; ++j) {
-                    const int32_t i = i0 + j * parts;
-                    got[j] = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-                    if (i <= sh.last) {
-                        const int64_t slot = (sh.Slot(i) * p.step_heads + kv_i) * kRows + row;
-                        const float2 ml = __ldcg(p.part_ml + slot);
-                        got[j] = {ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d))};
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < kTogether; ++j) acc.Add(got[j].m, got[j].l, got[j].o);
-            }
-            for (int32_t i = 1; i < min(parts, 32); i *= 2) {
-                Partial other;
-                other.m = __shfl_xor_sync(0xffffffffu, acc.m, i);
-                other.l = __shfl_xor_sync(0xffffffffu, acc.l, i);
-                other.o.x = __shfl_xor_sync(0xffffffffu, acc.o.x, i);
-                other.o.y = __shfl_xor_sync(0xffffffffu, acc.o.y, i);
-                other.o.z = __shfl_xor_sync(0xffffffffu, acc.o.z, i);
-                other.o.w = __shfl_xor_sync(0xffffffffu, acc.o.w, i);
-                acc.Add(other.m, other.l, other.o);
-            }
-            if (parts > 32) {
-                __syncthreads();
-                if (lane == 0) partials[warp] = acc;
-                __syncthreads();
-                if (part == 0) {
-                    for (int32_t i = 1; i < parts / 32; ++i) {
-                        const Partial other = partials[warp + i];
-                        acc.Add(other.m, other.l, other.o);
-                    }
-                }
-            }
-            if (live && part == 0) {
-                const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
-                if (d < p.pools.head_dim) {  // head_dim is a multiple of eight
-                    auto *to = reinterpret_cast<typename Half16<T>::Pair *>(reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim + d);
-                    to[0] = Half16<T>::FromFloat2(acc.o.x * inv, acc.o.y * inv);
-                    to[1] = Half16<T>::FromFloat2(acc.o.z * inv, acc.o.w * inv);
-                }
-                if (d == 0 && p.lse != nullptr) p.lse[head_at] = acc.l == 0.0f ? -INFINITY : (acc.m + Log2(acc.l)) * kLn2;
-            }
-        }
         return;
     }
-    if (!kScores) return;
+    FindStep(p, scan, p.units, w * per, &found);
+    const int32_t b = found.b;
+    const int32_t steps = SpanOf(p, b).steps;
+    const int64_t inside = w * per - found.before;
+    const int32_t unit = static_cast<int32_t>(Divide(inside, steps));
+    const int64_t into = inside - static_cast<int64_t>(unit) * steps;
+    if (into == 0) {  // nothing is cut here
+        asm volatile("griddepcontrol.wait;\n" ::: "memory");
+        return;
+    }
+    const Shares sh = SharesAt(w * per - into, steps, per);
+    const int32_t cuts = sh.last - sh.first, cut = w - sh.first - 1;
+    const int32_t kvg = unit / p.row_tiles, row_tile = unit - kvg * p.row_tiles;
+    const int32_t rows = min(kRows, p.group - row_tile * kRows);
+    const int64_t head0 = static_cast<int64_t>(b) * p.n_q_heads + kvg * p.step_heads * p.group + row_tile * kRows;
+    const int32_t fours = p.step_heads * rows * (kDim / 4);    // groups of four output elements
+    const int32_t mine = (fours + cuts - 1) / cuts;            // this block's
+    int32_t lanes = 1;                                         // thread groups per pass, a power of two
+    while (lanes < mine && lanes < kJoinThreads) lanes *= 2;
+    const int32_t parts = kJoinThreads / lanes;                // threads that share a group's shares
+    const int32_t at = tid / parts, part = tid % parts;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    for (int32_t base = 0; base < mine; base += lanes) {
+        const int32_t four = cut * mine + base + at;
+        const bool live = base + at < mine && four < fours;
+        const int32_t head_row = live ? four / (kDim / 4) : 0, d = live ? (four - head_row * (kDim / 4)) * 4 : 0;
+        const int32_t kv_i = head_row / rows, row = head_row - kv_i * rows;
+        const int64_t head_at = head0 + kv_i * p.group + row;
+        Partial acc = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+        constexpr int kTogether = 4;
+        for (int32_t i0 = sh.first + part; live && i0 <= sh.last; i0 += kTogether * parts) {
+            Partial got[kTogether];
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) {
+                const int32_t i = i0 + j * parts;
+                got[j] = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+                if (i <= sh.last) {
+                    const int64_t slot = (sh.Slot(i) * p.step_heads + kv_i) * kRows + row;
+                    const float2 ml = __ldcg(p.part_ml + slot);
+                    got[j] = {ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d))};
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) acc.Add(got[j].m, got[j].l, got[j].o);
+        }
+        for (int32_t i = 1; i < min(parts, 32); i *= 2) {
+            Partial other;
+            other.m = __shfl_xor_sync(0xffffffffu, acc.m, i);
+            other.l = __shfl_xor_sync(0xffffffffu, acc.l, i);
+            other.o.x = __shfl_xor_sync(0xffffffffu, acc.o.x, i);
+            other.o.y = __shfl_xor_sync(0xffffffffu, acc.o.y, i);
+            other.o.z = __shfl_xor_sync(0xffffffffu, acc.o.z, i);
+            other.o.w = __shfl_xor_sync(0xffffffffu, acc.o.w, i);
+            acc.Add(other.m, other.l, other.o);
+        }
+        if (parts > 32) {
+            __syncthreads();
+            if (lane == 0) partials[warp] = acc;
+            __syncthreads();
+            if (part == 0) {
+                for (int32_t i = 1; i < parts / 32; ++i) {
+                    const Partial other = partials[warp + i];
+                    acc.Add(other.m, other.l, other.o);
+                }
+            }
+        }
+        if (live && part == 0) {
+            const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
+            if (d < p.pools.head_dim) {  // head_dim is a multiple of eight
+                auto *to = reinterpret_cast<typename Half16<T>::Pair *>(reinterpret_cast<T *>(p.out) + head_at * p.pools.head_dim + d);
+                to[0] = Half16<T>::FromFloat2(acc.o.x * inv, acc.o.y * inv);
+                to[1] = Half16<T>::FromFloat2(acc.o.z * inv, acc.o.w * inv);
+            }
+            if (kScores && d == 0) p.whole_ml[head_at] = make_float2(acc.m, acc.l);
+            if (d == 0 && p.lse != nullptr) p.lse[head_at] = acc.l == 0.0f ? -INFINITY : (acc.m + Log2(acc.l)) * kLn2;
+        }
+    }
+}
 
-    // ---- weights: steps [at, end) of the batch's steps times weight heads
-    extern __shared__ float2 head_ml[];  // maximum and reciprocal sum of the query heads that count for a weight head
-    const int32_t block = blockIdx.x - p.workers;
+// Adds the attention every token received to its weight.  The steps of all sequences and weight heads are cut into equal
+// runs, one to a block; like the second kernel this one finds its work before it waits for the results.
+// kAtOnce tokens and kHeads heads of a thread have their loads in flight together.
+template <int kThreads, int kAtOnce, int kHeads>
+__global__ void __launch_bounds__(kThreads, 8) AddWeightsKernel(const __grid_constant__ AttendParams p) {
+    __shared__ int64_t scan_warp[kThreads / 32];
+    __shared__ Place64 found;
+    const uint32_t tid = threadIdx.x;
+    const StepScan scan = ScanSteps<kThreads>(p, scan_warp);
     const int64_t total = scan.all * p.n_weight_heads;
-    const int64_t share = Divide(total + weight_blocks - 1, weight_blocks);
-    int64_t at = block * share;
+    const int64_t share = Divide(total + gridDim.x - 1, gridDim.x);
+    int64_t at = blockIdx.x * share;
     const int64_t end = min(total, at + share);
     if (at >= end) return;
     FindStep(p, scan, p.n_weight_heads, at, &found);
     int32_t b = found.b;
-    int64_t before = found.before;  // of sequence b, all weight heads counted
+    Span span = SpanOf(p, b);
+    int32_t wh = static_cast<int32_t>(Divide(at - found.before, span.steps));
+    int32_t step0 = static_cast<int32_t>(at - found.before - static_cast<int64_t>(wh) * span.steps);
     const int32_t n_heads = p.n_weight_heads == 1 ? p.n_q_heads : p.group;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     while (at < end) {
-        const Span span = SpanOf(p, b);
-        if (span.steps == 0) {
-            ++b;
-            continue;
-        }
-        const int64_t inside = at - before;
-        const int32_t wh = static_cast<int32_t>(Divide(inside, span.steps));
-        const int32_t step0 = static_cast<int32_t>(inside - static_cast<int64_t>(wh) * span.steps);
         const int32_t steps = static_cast<int32_t>(min(static_cast<int64_t>(span.steps - step0), end - at));
-        const int32_t head0 = p.n_weight_heads == 1 ? 0 : wh * p.group;
-        const int64_t unit0 = Divide(before, p.n_weight_heads) * p.units;  // first step of the sequence, all units counted
-        // Where the shares of head0 + i lie, and its KV head and row in them.
-        auto shares_of = [&](int32_t i, int32_t &kv_i, int32_t &row) {
-            const int32_t kv = (head0 + i) / p.group, in_group = head0 + i - kv * p.group;
-            const int32_t kvg = kv / p.step_heads;
-            kv_i = kv - kvg * p.step_heads;
-            row = in_group % kRows;
-            return SharesAt(unit0 + (static_cast<int64_t>(kvg) * p.row_tiles + in_group / kRows) * span.steps, span.steps, per);
-        };
+        const int64_t head_at = static_cast<int64_t>(b) * p.n_q_heads + (p.n_weight_heads == 1 ? 0 : wh * p.group);
+        const float2 *stats = p.whole_ml + head_at;
         // a token on a page outside the pool was masked like any other: its score is negative infinity
-        const float *scores = p.scores + (static_cast<int64_t>(b) * p.n_q_heads + head0) * p.score_stride;
-        const float *w_in = p.weights + b * p.w_batch + wh * p.w_head;
-        float *w_out = p.weights_out + b * p.wo_batch + wh * p.wo_head;
-        const int32_t t_begin = step0 * p.step_tokens;  // relative to the span's base, as `last`
+        const float *scores = p.scores + head_at * p.score_stride;
+        const float *w_in = p.weights + b * p.w_batch + wh * p.w_head + span.base;
+        float *w_out = p.weights_out + b * p.wo_batch + wh * p.wo_head + span.base;
+        const int32_t skip = span.first - span.base;  // tokens of the first tile that lie before the window
         const int32_t last = min((step0 + steps) * p.step_tokens, span.len - span.base);
-        constexpr int kAtOnce = 4, kHeadsAtOnce = 4;  // tokens and heads of a thread whose loads are in flight together
-        for (int32_t t_block = t_begin; t_block < last; t_block += kAtOnce * kJoinThreads) {
-            const int32_t t0 = t_block + static_cast<int32_t>(tid);
-            float received[kAtOnce] = {}, old[kAtOnce] = {};
-            for (int32_t i0 = 0; i0 < n_heads; i0 += kHeadsAtOnce) {
-                float score[kHeadsAtOnce][kAtOnce];
+        for (int32_t t0 = step0 * p.step_tokens + static_cast<int32_t>(tid); t0 < last; t0 += kAtOnce * kThreads) {
+            float received[kAtOnce] = {}, old[kAtOnce];
 #pragma unroll
-                for (int h = 0; h < kHeadsAtOnce; ++h) {
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int32_t t = t0 + j * kThreads;
+                old[j] = t < last && t >= skip ? w_in[t] : 0.0f;
+            }
+#pragma unroll kHeads
+            for (int32_t i = 0; i < n_heads; ++i) {
+                const float2 ml = __ldcg(stats + i);
+                const float *row = scores + i * p.score_stride + t0;
+                float score[kAtOnce];
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; ++j) {
-                        score[h][j] = -INFINITY;
-                        if (i0 + h < n_heads && t0 + j * kJoinThreads < last) {
-                            score[h][j] = __ldcg(scores + (i0 + h) * p.score_stride + t0 + j * kJoinThreads);
-                        }
-                    }
-                }
-                if (i0 == 0) {
+                for (int j = 0; j < kAtOnce; ++j) score[j] = t0 + j * kThreads < last ? __ldcg(row + j * kThreads) : -INFINITY;
+                const float top = ml.x == -INFINITY ? 0.0f : ml.x, inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; ++j) {
-                        const int32_t t = span.base + t0 + j * kJoinThreads;
-                        if (t0 + j * kJoinThreads < last && t >= span.first) old[j] = w_in[t];
-                    }
-                    if (t_block == t_begin) {
-                        // maximum and sum of every head that counts here, of few shares by a thread, of many by a warp
-                        __syncthreads();
-                        const int32_t by = span.steps > 6 * per ? 32 : 1;
-                        for (int32_t i = static_cast<int32_t>(tid) / by; i < n_heads; i += kJoinThreads / by) {
-                            int32_t kv_i, row;
-                            const Shares sh = shares_of(i, kv_i, row);
-                            float2 ml;
-                            if (sh.first == sh.last) {
-                                ml = __ldcg(p.whole_ml + static_cast<int64_t>(b) * p.n_q_heads + head0 + i);
-                            } else {
-                                ml = StatsOf(p, sh, kv_i, row, kRows, sh.first + static_cast<int32_t>(tid) % by, by);
-                            }
-                            if (by == 32 && sh.first != sh.last) {
-#pragma unroll
-                                for (int d = 16; d > 0; d /= 2) {
-                                    const float m2 = __shfl_xor_sync(0xffffffffu, ml.x, d), l2 = __shfl_xor_sync(0xffffffffu, ml.y, d);
-                                    const float grown = fmaxf(ml.x, m2);
-                                    const float use = grown == -INFINITY ? 0.0f : grown;
-                                    ml.y = ml.y * Exp2(ml.x - use) + l2 * Exp2(m2 - use);
-                                    ml.x = grown;
-                                }
-                            }
-                            if (tid % by == 0) {
-                                head_ml[i] = make_float2(ml.x == -INFINITY ? 0.0f : ml.x, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
-                            }
-                        }
-                        __syncthreads();
-                    }
-                }
-#pragma unroll
-                for (int h = 0; h < kHeadsAtOnce; ++h) {
-                    if (i0 + h < n_heads) {
-                        const float2 ml = head_ml[i0 + h];
-#pragma unroll
-                        for (int j = 0; j < kAtOnce; ++j) received[j] += Exp2(score[h][j] - ml.x) * ml.y;
-                    }
-                }
+                for (int j = 0; j < kAtOnce; ++j) received[j] += Exp2(score[j] - top) * inv;
             }
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
-                const int32_t t = span.base + t0 + j * kJoinThreads;
-                if (t0 + j * kJoinThreads < last && t >= span.first) w_out[t] = old[j] + received[j];
+                const int32_t t = t0 + j * kThreads;
+                if (t < last && t >= skip) w_out[t] = old[j] + received[j];
             }
         }
         at += steps;
-        if (at == before + static_cast<int64_t>(span.steps) * p.n_weight_heads) {
-            before = at;
-            ++b;
+        step0 = 0;
+        if (++wh == p.n_weight_heads && at < end) {
+            wh = 0;
+            do {
+                span = SpanOf(p, ++b);
+            } while (span.steps == 0);
         }
     }
 }
@@ -919,25 +868,30 @@ void LaunchAttend(AttendParams p, cudaStream_t stream) {
     using Shape = AttendShape<kDim, kScores>;
     static_assert((Shape::kRingBytes + 2048) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
     auto *main_kernel = AttendPagesKernel<T, kDim, kRows, kScores>;
-    auto *join_kernel = JoinSharesKernel<T, kDim, kRows, kScores>;
     EnsureDynamicSmem(main_kernel, Shape::kRingBytes);
     const int32_t sm_count = GetDeviceInfo().sm_count;
     p.workers = std::min(kMaxWorkers, sm_count * Shape::kCtasPerSm);
     main_kernel<<<p.workers, kAttendThreads, Shape::kRingBytes, stream>>>(p);
 
-    // The second kernel's blocks wait on the device for the first kernel's end, their launch overlaps it.
-    const int32_t weight_blocks = kScores ? 5 * sm_count : 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.workers + weight_blocks);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.dynamicSmemBytes = kScores ? static_cast<size_t>(p.n_weight_heads == 1 ? p.n_q_heads : p.group) * 8 : 0;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, join_kernel, p, weight_blocks);
+    // The kernels that follow wait on the device for the one before them; their launch overlaps it.
+    auto launch_after = [&](auto kernel, int32_t blocks) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<uint32_t>(blocks));
+        cfg.blockDim = dim3(kJoinThreads);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, kernel, p);
+    };
+    launch_after(JoinSharesKernel<T, kDim, kRows, kScores>, p.workers);
+    if (kScores) {
+        // loads in flight over tokens, or over heads where all query heads count for one weight
+        const bool many_heads = p.n_weight_heads == 1 && p.n_q_heads >= 8;
+        launch_after(many_heads ? AddWeightsKernel<kJoinThreads, 1, 8> : AddWeightsKernel<kJoinThreads, 4, 4>, 8 * sm_count);
+    }
 }
 
 template <typename T, int kDim>
