@@ -222,6 +222,10 @@ def _check_attend(q, k_pool, v_pool, table, lens, dtype, window=0, scale=None, *
     ([77, 150], 4, 2, 128, 2, "hnd", 20),
     ([333], 4, 2, 136, 1, "nhd", 0),
     ([333, 70], 4, 2, 200, 12, "nhd", 69),
+    ([700, 13, 0, 260], 32, 8, 64, 16, "nhd", 0),               # steps of two heads
+    ([700, 13, 0, 260], 48, 4, 80, 16, "nhd", 0),               # of four, sixteen-row tiles
+    ([700, 13, 0, 260], 12, 12, 96, 64, "nhd", 100),
+    ([9000], 68, 4, 80, 5, "nhd", 0),                           # seventeen heads to a group: two row tiles
 ])
 def test_attend_matches_the_definition(lens, hq, hkv, dim, page, layout, window, dtype):
     case = _attend_case(sum(lens) + dim, lens, hq, hkv, dim, dtype, page, layout)
@@ -235,6 +239,8 @@ def test_attend_matches_the_definition(lens, hq, hkv, dim, page, layout, window,
     ([3000, 10], 18, 1, 128, 100),
     ([1200, 513, 100], 20, 2, 80, 700),
     ([20000], 8, 1, 64, 0),
+    ([5000, 77, 3], 24, 8, 64, 0),
+    ([5000, 77, 3], 40, 4, 80, 333),
 ])
 def test_attend_accumulates_weights(lens, hq, hkv, dim, window, heads):
     q, k_pool, v_pool, table, n = _attend_case(sum(lens), lens, hq, hkv, dim, "bf16")
