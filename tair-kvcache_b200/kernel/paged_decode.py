@@ -79,6 +79,11 @@ def _layout(t: Optional[torch.Tensor]):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
+def _layouts(flat):
+    """Layouts whose four fields stand one after the other (a lookup key is made faster that way)."""
+    return [flat[i:i + 4] for i in range(0, len(flat), 4)]
+
+
 def _pools(k, v):
     """The fields of kvcm_b200_kv_pools_t behind the two addresses, from the pools' layouts."""
     (shape, strides, dtype, device) = k
@@ -184,7 +189,8 @@ def _workspace_bytes(name: str, size: int) -> int:
 
 
 @functools.lru_cache(maxsize=_REMEMBERED)
-def _append_plan(query, key, value, positions, slots, k, v, inv_freq, query_out):
+def _append_plan(query, query_out, *flat):
+    key, value, positions, slots, k, v, inv_freq = _layouts(flat)
     pools = _pools(k, v)
     tokens = key[0][0] if len(key[0]) else 0
     k_args, v_args = _heads(key, "key", k, tokens), _heads(value, "value", k, tokens)
@@ -230,13 +236,16 @@ def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, valu
     if not isinstance(slot_indices, torch.Tensor):
         slot_indices = _index_tensor(slot_indices, k_pool.device)
     pools, tokens, q_args, q_out_args, k_args, v_args, position_bytes, slot_bytes, rotary_dim, device = _append_plan(
-        _layout(query), _layout(key), _layout(value), _layout(positions), _layout(slot_indices), _layout(k_pool),
-        _layout(v_pool), _layout(inv_freq), _layout(query_out))
+        _layout(query), _layout(query_out), key.shape, key.stride(), key.dtype, key.device, value.shape, value.stride(),
+        value.dtype, value.device, positions.shape, positions.stride(), positions.dtype, positions.device, slot_indices.shape,
+        slot_indices.stride(), slot_indices.dtype, slot_indices.device, k_pool.shape, k_pool.stride(), k_pool.dtype,
+        k_pool.device, v_pool.shape, v_pool.stride(), v_pool.dtype, v_pool.device, inv_freq.shape, inv_freq.stride(),
+        inv_freq.dtype, inv_freq.device)
     if q_args is None:
         q_all = (0, 0, 0, 0, 0, 0, 0)
     else:
         if query_out is None:
-            query_out = query.new_empty(query.shape)
+            query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
         q_all = (query.data_ptr(), *q_args, query_out.data_ptr(), *q_out_args)
     _launch("kvcm_b200_append_pages", device, (k_pool.data_ptr(), v_pool.data_ptr(), *pools), *q_all, key.data_ptr(), *k_args,
             value.data_ptr(), *v_args, positions.data_ptr(), position_bytes, slot_indices.data_ptr(), slot_bytes, tokens,
@@ -245,7 +254,8 @@ def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, valu
 
 
 @functools.lru_cache(maxsize=_REMEMBERED)
-def _attend_plan(query, k, v, table, lens, window, out, lse, weights, weights_out):
+def _attend_plan(window, out, lse, weights, weights_out, *flat):
+    query, k, v, table, lens = _layouts(flat)
     pools = _pools(k, v)
     batch, width, table_stride = _sequences(table, lens, k)
     q_args = _heads(query, "query", k, batch)
@@ -290,10 +300,13 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     them - what batch_evict_kv_pages ranks by.  Entries that are not attended are left as they are."""
     _no_grad(query, k_pool, v_pool, weights)
     pools, q_args, table_args, w_args, wo_args, size, default_scale, device = _attend_plan(
-        _layout(query), _layout(k_pool), _layout(v_pool), _layout(block_table), _layout(context_lens), int(window),
-        _layout(out), _layout(lse), _layout(weights), _layout(weights_out))
+        int(window), out if out is None else _layout(out), lse if lse is None else _layout(lse),
+        weights if weights is None else _layout(weights), weights_out if weights_out is None else _layout(weights_out),
+        query.shape, query.stride(), query.dtype, query.device, k_pool.shape, k_pool.stride(), k_pool.dtype, k_pool.device,
+        v_pool.shape, v_pool.stride(), v_pool.dtype, v_pool.device, block_table.shape, block_table.stride(), block_table.dtype,
+        block_table.device, context_lens.shape, context_lens.stride(), context_lens.dtype, context_lens.device)
     if out is None:
-        out = query.new_empty(query.shape)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     w_all = (0, 0, 0, 0, 0, 0, 0)
     if w_args is not None:
         w_all = (weights.data_ptr(), *w_args[:2], (weights if weights_out is None else weights_out).data_ptr(), *wo_args)
@@ -306,7 +319,8 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
 
 
 @functools.lru_cache(maxsize=_REMEMBERED)
-def _evict_plan(k, v, table, lens, weights, positions, budget, recent, weights_out, positions_out):
+def _evict_plan(budget, recent, weights_out, positions_out, *flat):
+    k, v, table, lens, weights, positions = _layouts(flat)
     pools = _pools(k, v)
     batch, width, table_stride = _sequences(table, lens, k)
     tokens = width * pools[4]
@@ -346,9 +360,13 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     the pool is left out and counted in `status`, as is a length beyond the table (cut to it)."""
     _no_grad(k_pool, v_pool, weights)
     pools, table_args, batch, sizes, w_args, p_args, wo_args, po_args, size, device = _evict_plan(
-        _layout(k_pool), _layout(v_pool), _layout(block_table), _layout(context_lens), _layout(weights), _layout(positions),
-        int(budget), int(recent), _layout(weights_out), _layout(positions_out))
-    new_lens = context_lens.new_empty(batch)
+        int(budget), int(recent), weights_out if weights_out is None else _layout(weights_out),
+        positions_out if positions_out is None else _layout(positions_out), k_pool.shape, k_pool.stride(), k_pool.dtype,
+        k_pool.device, v_pool.shape, v_pool.stride(), v_pool.dtype, v_pool.device, block_table.shape, block_table.stride(),
+        block_table.dtype, block_table.device, context_lens.shape, context_lens.stride(), context_lens.dtype,
+        context_lens.device, weights.shape, weights.stride(), weights.dtype, weights.device, positions.shape,
+        positions.stride(), positions.dtype, positions.device)
+    new_lens = torch.empty_like(context_lens)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
     _launch("kvcm_b200_evict_pages", device, (k_pool.data_ptr(), v_pool.data_ptr(), *pools), batch, block_table.data_ptr(),
             *table_args, context_lens.data_ptr(), *sizes, weights.data_ptr(), *w_args, positions.data_ptr(), *p_args,
