@@ -825,7 +825,10 @@ __global__ void __launch_bounds__(kThreads, 8) AddWeightsKernel(const __grid_con
     const int64_t share = Divide(total + gridDim.x - 1, gridDim.x);
     int64_t at = blockIdx.x * share;
     const int64_t end = min(total, at + share);
-    if (at >= end) return;
+    if (at >= end) {  // what follows in the stream relies on every block having waited
+        asm volatile("griddepcontrol.wait;\n" ::: "memory");
+        return;
+    }
     FindStep(p, scan, p.n_weight_heads, at, &found);
     int32_t b = found.b;
     Span span = SpanOf(p, b);

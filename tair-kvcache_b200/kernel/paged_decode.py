@@ -232,7 +232,7 @@ def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, valu
     page * page_tokens + offset, the numbers batch_scatter_kv_caches takes; -1 marks a padding token, which writes
     nothing; any other slot outside the pool is skipped and counted in `status` (four zeroed 32-bit words on the GPU).
     The same slot twice in one call is a data race.  `query_out` may be `query`."""
-    _no_grad(query, key, value, inv_freq)
+    _no_grad(query, key, value, inv_freq, k_pool, v_pool)
     if not isinstance(slot_indices, torch.Tensor):
         slot_indices = _index_tensor(slot_indices, k_pool.device)
     pools, tokens, q_args, q_out_args, k_args, v_args, position_bytes, slot_bytes, rotary_dim, device = _append_plan(

@@ -578,6 +578,67 @@ def test_pools_in_one_tensor_and_behind_four_gigabytes():
     assert torch.equal(_bits(k_pool[pages - 1, page - 1]), _bits(key[0])) and torch.equal(_bits(v_pool[0, 3]), _bits(key[1]))
 
 
+def test_nothing_to_do():
+    """Empty batches, block tables without pages, sequences without tokens: results are written all the same."""
+    k_pool = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device=DEV)
+    v_pool = torch.zeros_like(k_pool)
+
+    def i32(*shape):
+        return torch.zeros(shape, dtype=torch.int32, device=DEV)
+
+    for b, width in ((0, 3), (0, 0), (3, 0), (3, 2), (3, 9)):  # of the last two one is cut into runs, one is not
+        q = torch.ones(b, 4, 64, dtype=torch.bfloat16, device=DEV)
+        out, lse = torch.full_like(q, 7.0), torch.full((b, 4), 7.0, device=DEV)
+        w = torch.full((b, 2, width * 16), 3.0, device=DEV)
+        batch_attend_kv_pages(q, k_pool, v_pool, i32(b, width), i32(b), out=out, lse=lse, weights=w)
+        assert (out == 0).all() and (lse == -math.inf).all() and (w == 3.0).all()
+        pos = i32(b, 2, width * 16)
+        lens = batch_evict_kv_pages(k_pool, v_pool, i32(b, width), i32(b), w, pos, 5, 2)
+        assert lens.shape == (b,) and (lens == 0).all() and (w == 3.0).all() and (pos == 0).all()
+        # lengths beyond an empty table are cut to nothing
+        if b and not width:
+            status = _status()
+            lens = batch_evict_kv_pages(k_pool, v_pool, i32(b, 0), i32(b) + 9, w, pos, 5, 2, status=status)
+            assert (lens == 0).all() and status.tolist()[:2] == [b, b]
+
+
+def test_many_calls_in_a_row_read_what_the_one_before_wrote():
+    """Kernels of one call start before the one in front has ended: the chain append, attend, evict without any
+    synchronisation gives what it gives with one after every call."""
+    gen = torch.Generator().manual_seed(4)
+    hq, hkv, dim, width = 8, 2, 64, 24
+    results = []
+    for sync in (True, False):
+        gen.manual_seed(4)
+        k_pool, v_pool = (t.to(DEV) for t in oracle.make_pools(gen, 4 * width + 1, 16, hkv, dim, "bf16"))
+        table = torch.randperm(4 * width, generator=gen).to(torch.int32).view(4, width).to(DEV)
+        lens = torch.tensor([384, 200, 383, 10], dtype=torch.int32, device=DEV) - 30
+        weights = torch.rand(4, hkv, width * 16, generator=gen).to(DEV)
+        positions = torch.arange(width * 16, dtype=torch.int32).expand(4, hkv, -1).contiguous().to(DEV)
+        inv_freq, _ = rotary_frequencies(dim, device=DEV)
+        row = torch.arange(4, device=DEV)
+        outs = []
+        for step in range(30):
+            qkv = torch.randn(4, hq + 2 * hkv, dim, generator=gen).to(torch.bfloat16).to(DEV)
+            at = lens.long().clamp_max(width * 16 - 1)
+            slots = table[row, at // 16].long() * 16 + at % 16
+            positions[row, :, at] = 1000 + step
+            q = batch_append_kv_pages(qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:], at, slots, k_pool, v_pool, inv_freq)
+            if sync:
+                torch.cuda.synchronize()
+            lens = (lens + 1).clamp_max(width * 16)
+            outs.append(batch_attend_kv_pages(q, k_pool, v_pool, table, lens, weights=weights))
+            if sync:
+                torch.cuda.synchronize()
+            lens = batch_evict_kv_pages(k_pool, v_pool, table, lens, weights, positions, 190, 20)
+            if sync:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append([_bits(torch.stack(outs)), weights, positions, _bits(k_pool), _bits(v_pool), lens])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_refusals_on_the_device():
     k_pool, v_pool, table, n, w, pos = _evict_case(2, [64], 2, 2, 64)
     dk, dv, dt, dn = k_pool.to(DEV), v_pool.to(DEV), table.to(DEV), n.to(DEV)
