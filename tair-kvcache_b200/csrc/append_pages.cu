@@ -24,16 +24,6 @@ constexpr int kAppendItems = 1;  // items a thread has in flight
 constexpr int kMaxAppendHeadDim = 1024;
 constexpr int kMaxAppendTokens = 4;  // of a CTA
 
-// n / d for 32-bit numbers by one wide multiplication: magic = floor(2^64 / d) + 1 (0 for d = 1) is exact for all of them.
-struct FastDivide {
-    uint64_t magic;
-    uint32_t d;
-    FastDivide(uint32_t by = 1) : magic(by <= 1 ? 0 : ~uint64_t{0} / by + 1), d(by < 1 ? 1 : by) {}
-    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
-        return magic == 0 ? n : static_cast<uint32_t>(__umul64hi(n, magic));
-    }
-};
-
 struct HeadRows {
     const void *src;
     void *dst;

@@ -58,8 +58,9 @@ struct EvictParams {
     int32_t n_heads;         // weight heads
     int32_t heads_per_move;  // KV heads that move together
     int32_t budget, recent;
-    int32_t chunks;  // 16-byte pieces of a row
     int32_t separate_out;
+    FastDivide pieces;       // 16-byte pieces of one move: K and V rows of every head that moves
+    FastDivide row_pieces;   // of a row
     int32_t units;           // batch * weight heads
     int32_t moves_at_once;   // of a block of the second kernel
     int32_t blocks_per_unit;
@@ -394,7 +395,6 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
 __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_constant__ EvictParams p) {
     __shared__ int64_t from_row[kMaxMovesAtOnce], to_row[kMaxMovesAtOnce];
     const uint32_t tid = threadIdx.x;
-    const uint32_t pieces = 2u * p.chunks * p.heads_per_move;  // of one move: K and V rows of every head that moves
     const int64_t blocks = static_cast<int64_t>(p.units) * p.blocks_per_unit;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_con
             pos_out[m.x] = -1;
         }
         __syncthreads();
-        const uint32_t n_pieces = static_cast<uint32_t>(here) * pieces;
+        const uint32_t n_pieces = static_cast<uint32_t>(here) * p.pieces.d;
         constexpr int kUnroll = 8;
         for (uint32_t base = tid; base < n_pieces; base += kMoveThreads * kUnroll) {
             uint4 data[kUnroll];
@@ -442,11 +442,11 @@ __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_con
                 const uint32_t f = base + u * kMoveThreads;
                 to[u] = nullptr;
                 if (f < n_pieces) {
-                    const uint32_t m = f / pieces;
-                    const uint32_t within = f - m * pieces;
-                    const uint32_t row = within / p.chunks;
+                    const uint32_t m = p.pieces(f);
+                    const uint32_t within = f - m * p.pieces.d;
+                    const uint32_t row = p.row_pieces(within);
                     const int64_t off = static_cast<int64_t>(row >> 1) * p.pools.head_stride +
-                                        static_cast<int64_t>(within - row * p.chunks) * 16;
+                                        static_cast<int64_t>(within - row * p.row_pieces.d) * 16;
                     uint8_t *pool = (row & 1) ? p.pools.v : p.pools.k;
                     if (from_row[m] >= 0) {
                         data[u] = __ldcs(reinterpret_cast<const uint4 *>(pool + from_row[m] + off));
@@ -525,7 +525,7 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     }
     if (!HaveDevice()) return KVCM_ER_NO_DEVICE;
     if (batch == 0) return KVCM_OK;
-    EvictParams p = {};
+    EvictParams p{};
     p.pools = AsPagedPools(*pools);
     p.table = d_block_table;
     p.lens = d_context_lens;
@@ -552,7 +552,8 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     p.heads_per_move = n_weight_heads == 1 ? pools->n_kv_heads : 1;
     p.budget = budget;
     p.recent = recent;
-    p.chunks = pools->head_dim / 8;
+    p.row_pieces = FastDivide(static_cast<uint32_t>(pools->head_dim / 8));
+    p.pieces = FastDivide(2 * p.row_pieces.d * static_cast<uint32_t>(p.heads_per_move));
     p.separate_out = d_weights_out != d_weights || d_positions_out != d_positions;
 
     // As many CTAs as fit two to an SM, but none with fewer than about a thousand slots, and slices that fit shared memory.
@@ -565,8 +566,7 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     const bool cached = slice <= kMaxCachedSlots;
     p.units = static_cast<int32_t>(units);
     p.n_moves = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(d_workspace) + EvictMovesBytes(units, table_tokens, budget));
-    const int32_t pieces = 2 * p.chunks * p.heads_per_move;
-    p.moves_at_once = std::min(kMaxMovesAtOnce, std::max(1, kMovePieces / pieces));
+    p.moves_at_once = std::min(kMaxMovesAtOnce, std::max(1, kMovePieces / static_cast<int>(p.pieces.d)));
     p.blocks_per_unit = static_cast<int32_t>((p.max_moves + p.moves_at_once - 1) / p.moves_at_once);
 
     cudaLaunchConfig_t cfg = {};

@@ -56,6 +56,16 @@ inline bool RowsAre16ByteAligned(const kvcm_b200_kv_pools_t &p) {
            ((p.page_stride | p.token_stride | p.head_stride | p.head_dim) & 7) == 0;
 }
 
+// n / d for 32-bit numbers by one wide multiplication: magic = floor(2^64 / d) + 1 (0 for d = 1) is exact for all of them.
+struct FastDivide {
+    uint64_t magic;
+    uint32_t d;
+    FastDivide(uint32_t by = 1) : magic(by <= 1 ? 0 : ~uint64_t{0} / by + 1), d(by < 1 ? 1 : by) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        return magic == 0 ? n : static_cast<uint32_t>(__umul64hi(n, magic));
+    }
+};
+
 // status[0] += count, status[1] = max(status[1], 1 + number of the offending token or sequence).
 __device__ __forceinline__ void CountSkipped(uint32_t *status, uint32_t number, uint32_t count) {
     if (status != nullptr) {
