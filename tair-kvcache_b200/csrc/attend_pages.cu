@@ -55,8 +55,8 @@ struct AttendParams {
     int64_t w_batch, w_head, wo_batch, wo_head;
     int32_t n_weight_heads;
     // workspace
-    float *part_o;          // [workers * 2][step_heads][rows][dim]
-    float2 *part_ml;        // [workers * 2][step_heads][rows] maximum and sum of a share, the maximum in units of log2
+    float *part_o;          // [step_heads * kRows][dim / 16][2 * workers][16]: a join reads many shares of a few elements
+    float2 *part_ml;        // [step_heads * kRows][2 * workers] maximum and sum of a share, the maximum in units of log2
     float2 *whole_ml;       // [batch][n_q_heads] maximum and sum of whole heads; with weights only
     float *scores;          // [batch][n_q_heads][score_stride], in units of log2; null without weights
     int64_t score_stride;
@@ -68,6 +68,7 @@ struct AttendParams {
     int32_t kv_groups;   // KV heads / step_heads
     int32_t units;       // kv_groups * row_tiles
     int32_t k_steps;     // 16-element pieces of a row that are not padding
+    int64_t v_minus_k;   // bytes from a row of K to the same of V
     int64_t copy_stride; // bytes between the rows that one copy instruction after another takes
     int32_t table_tokens;
     int32_t window;
@@ -97,6 +98,11 @@ __device__ __forceinline__ Span SpanOf(const AttendParams &p, int32_t b) {
 // a / b, in 32 bits where they do: a 64-bit division takes several times as long.
 __device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
     return (a | b) <= 0xffffffffll ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// Where a share's entry of a line of entries lies, one per slot.
+__device__ __forceinline__ int64_t PartAt(int32_t line, int32_t slot, int32_t workers) {
+    return static_cast<int64_t>(line) * (2 * workers) + slot;
 }
 
 // Steps per run, the same in both kernels.
@@ -366,10 +372,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
 
     const uint32_t tiles_at = ring + warp * 2 * Shape::kTileBytes;
     const uint32_t copy_piece = lane % kPieces, copy_row = lane / kPieces;
-    const uint32_t copy_bytes = copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? 16u : 0u;
     const uint32_t copy_to = copy_row * Shape::kRowBytes + ((copy_piece ^ copy_row) * 16);  // of the first copy
-    const int64_t copy_from = static_cast<int64_t>(copy_row) * p.pools.token_stride + (copy_bytes != 0 ? copy_piece * 16 : 0);
-    const int64_t v_minus_k = p.pools.v - p.pools.k;
+    const int64_t copy_from = static_cast<int64_t>(copy_row) * p.pools.token_stride + (copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? copy_piece * 16 : 0);
     // Starts the copies of this warp's tile of the next step; rows that take no part become zeros, so that whatever lies
     // there cannot reach a product.
     auto load_tile = [&](int to_stage) {
@@ -381,6 +385,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
         const int64_t head_off = static_cast<int64_t>(ask.kvg * p.step_heads + my_head) * p.pools.head_stride;
         const uint32_t to = tiles_at + to_stage * Shape::kStageBytes + copy_to;
         const uint64_t policy = ReadOncePolicy();
+        const uint32_t copy_bytes = copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? 16u : 0u;
         if (p.whole_tiles) {
             if (!page_ok) valid = 0;
             if (valid != 0) {
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
                     const uint32_t bytes = (valid >> row) & 1u ? copy_bytes : 0u;
                     const uint32_t at = (to ^ (((i * kCopyRows) & 7) * 16)) + i * kCopyRows * Shape::kRowBytes;
                     CopyAsync16(at, from, bytes, policy);
-                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes, policy);
+                    CopyAsync16(at + Shape::kTileBytes, from + p.v_minus_k, bytes, policy);
                     from += p.copy_stride;
                 }
             }
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
                     const uint8_t *from = p.pools.k + (bytes != 0 ? row_off + copy_piece * 16 : 0);
                     const uint32_t at = (to ^ (((i * kCopyRows) & 7) * 16)) + i * kCopyRows * Shape::kRowBytes;
                     CopyAsync16(at, from, bytes, policy);
-                    CopyAsync16(at + Shape::kTileBytes, from + v_minus_k, bytes, policy);
+                    CopyAsync16(at + Shape::kTileBytes, from + p.v_minus_k, bytes, policy);
                 }
             }
         }
@@ -633,15 +638,18 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
                 }
             }
             __syncthreads();
-            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (begins_run ? 0 : 1)) * p.step_heads * kRows;
+            const int32_t slot = blockIdx.x + (begins_run ? 0 : p.workers);
+#pragma unroll 1  // few rounds, and registers are short
             for (int32_t i = tid; i < p.step_heads * rows * (kDim / 2); i += kAttendThreads) {
                 const int32_t head_row = i / (kDim / 2), kv_i = head_row / rows, row = head_row - kv_i * rows;
                 const int32_t d = (i - head_row * (kDim / 2)) * 2;
                 float m = -INFINITY;
+#pragma unroll 1
                 for (int32_t w = kv_i * token_tiles; w < (kv_i + 1) * token_tiles; ++w) m = fmaxf(m, join_ml[w][row].x);
                 const float use = m == -INFINITY ? 0.0f : m;
                 float l = 0.0f;
                 float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll 1
                 for (int32_t w = kv_i * token_tiles; w < (kv_i + 1) * token_tiles; ++w) {
                     const float2 ml = join_ml[w][row];
                     const float f = Exp2(ml.x - use);
@@ -663,9 +671,9 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
                         if (p.lse != nullptr) p.lse[head_at] = l == 0.0f ? -INFINITY : (m + Log2(l)) * kLn2;
                     }
                 } else {
-                    const int64_t to = slot + kv_i * kRows + row;
-                    *reinterpret_cast<float2 *>(p.part_o + to * kDim + d) = acc;
-                    if (d == 0) p.part_ml[to] = make_float2(m, l);
+                    const int32_t part_row = kv_i * kRows + row;
+                    *reinterpret_cast<float2 *>(p.part_o + PartAt(part_row * (kDim / 16) + d / 16, slot, p.workers) * 16 + d % 16) = acc;
+                    if (d == 0) p.part_ml[PartAt(part_row, slot, p.workers)] = make_float2(m, l);
                 }
             }
             __syncthreads();  // the sums may be overwritten
@@ -679,11 +687,12 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
     CopyWait<0>();
 }
 
-// Where the shares of a unit lie: runs [first, last]; the share of run w is in slot 2 w + (the unit begins within the run).
+// Where the shares of a unit lie: runs [first, last]; the share of run w is in slot w, or workers + w where the unit begins
+// within the run: consecutive runs in consecutive slots.
 struct Shares {
     int64_t t0, per;
     int32_t first, last;
-    __device__ __forceinline__ int64_t Slot(int32_t w) const { return 2 * static_cast<int64_t>(w) + (t0 > w * per ? 1 : 0); }
+    __device__ __forceinline__ int32_t Slot(int32_t w, int32_t workers) const { return w + (t0 > w * per ? workers : 0); }
 };
 
 __device__ __forceinline__ Shares SharesAt(int64_t t0, int64_t steps, int64_t per) {
@@ -770,9 +779,10 @@ __global__ void __launch_bounds__(kJoinThreads, 8) JoinSharesKernel(const __grid
                 const int32_t i = i0 + j * parts;
                 got[j] = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
                 if (i <= sh.last) {
-                    const int64_t slot = (sh.Slot(i) * p.step_heads + kv_i) * kRows + row;
-                    const float2 ml = __ldcg(p.part_ml + slot);
-                    got[j] = {ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(p.part_o + slot * kDim + d))};
+                    const int32_t slot = sh.Slot(i, p.workers), part_row = kv_i * kRows + row;
+                    const float2 ml = __ldcg(p.part_ml + PartAt(part_row, slot, p.workers));
+                    const float *from = p.part_o + PartAt(part_row * (kDim / 16) + d / 16, slot, p.workers) * 16 + d % 16;
+                    got[j] = {ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(from))};
                 }
             }
 #pragma unroll
@@ -1043,6 +1053,7 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.kv_groups = pools->n_kv_heads / p.step_heads;
     p.units = p.kv_groups * p.row_tiles;
     p.k_steps = (pools->head_dim + 15) / 16;
+    p.v_minus_k = p.pools.v - p.pools.k;
     // steps are counted in 64 bits over the batch and in 32 within a CTA's run
     if (static_cast<double>(batch) * p.units * (static_cast<double>(table_tokens) / p.step_tokens + 1 + kUnitCost) >= 1e11) {
         return KVCM_EC_OUT_OF_LIMIT;
