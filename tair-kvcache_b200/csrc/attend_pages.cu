@@ -7,23 +7,28 @@
 // share the KV head, 2 to 32 multiplications per byte.  One pass with a running maximum and sum.
 //
 // Four warps to a CTA, each with a ring of its own: tiles of 16 tokens of one KV head come from HBM by 16-byte asynchronous
-// copies, issued by the warp two tiles ahead, the table entry of the one after those already on its way; then
+// copies, issued by the warp one to three tiles ahead, the table entry of the one after those already on its way; then
 // ldmatrix, 16x8x16 matrix instructions whose 16 rows are the group's query heads, softmax in registers, and the product
-// with V.  No warp waits for another until a head is complete.  (TMA tile loads were measured in two forms and left:
-// with a producer warp for the CTA, 65 cycles to issue each box set the pace, 1050 to 1700 for a step of four tiles; with
-// every warp loading its own tile, the four barrier operations a tile needs, about 100 cycles each, did.)  A group is
-// far too small for the 128 rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
+// with V.  No warp waits for another until a head is complete.  (TMA tile loads were measured in three forms and left:
+// with producer warps, 65 cycles to issue each box set the pace, 1050 to 1700 for a step of four tiles; with every warp
+// loading its own tile, the four barrier operations a tile needs, about 100 cycles each, did.)  A group is far too
+// small for the 128 rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
 //
 // Probabilities enter the second product as two 16-bit halves, p = hi + lo, whose sum carries 16 (bf16) or more bits,
 // so the output is rounded once.  With a group of at most eight the halves cost nothing: hi takes rows 0-7 of the
 // matrix instruction, lo the rows 8-15 that the group leaves free.
 //
-// The work is cut by tokens, not by sequences: the steps (four tiles of one sequence) of the whole
-// batch are numbered through, and each of the persistent CTAs takes an equal run of them, found from the lengths on the
-// device.  Finishing a head costs about as much as two steps, so two are added to each that no one has to do: without them
-// the CTAs that took many short sequences finished last (37 sequences of 1 to 5000 tokens: 33 us instead of 27).  A head that lies within one run is finished there; the runs of a head that is cut leave their unnormalised
-// sums and statistics in the workspace, and the second kernel joins them, in order, so results do not depend on timing.
-// A third adds up the weights, which need every head's final statistics.
+// The work is cut by tokens, not by sequences: the steps (four tiles of one sequence) of the whole batch are numbered
+// through, and each of the persistent CTAs takes an equal run of them, found from the lengths on the device.  Finishing a
+// head costs about as much as two steps, so two are added to each that no one has to do: without them the CTAs that took
+// many short sequences finished last (37 sequences of 1 to 5000 tokens: 33 us instead of 27).  A head that lies within
+// one run is finished there; the runs of a head that is cut leave their unnormalised sums and statistics in the
+// workspace, and the second kernel joins them, in order, so results do not depend on timing.  A third adds up the
+// weights, which need every head's final statistics.
+//
+// 64 sequences of 512 to 8192 tokens, 32 query and 8 KV heads of 128, bf16: 173 us, 6.6 TB/s, 101 % of a plain copy.  One
+// sequence of 131,072 tokens on one KV head: 21.6 us, of which 10.3 are its bytes; 16 of 2000 to 6001 tokens with weights:
+// 55 us, of which 41.
 #include "paged_kv.cuh"
 
 namespace kvcm {
@@ -33,7 +38,7 @@ constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kTile = 16;                                  // tokens of a tile
 constexpr int kUnitCost = 2;                               // steps that finishing a unit takes about as long as
-constexpr int kUncutSteps = 4;
+constexpr int kUncutSteps = 4;                             // of a unit that stays whole whatever the batch
 constexpr int kMaxWorkers = 512;
 constexpr int kMaxAttendHeadDim = 256;
 constexpr int kJoinThreads = 128;
@@ -176,13 +181,13 @@ __device__ __forceinline__ float Log2(float x) {
     asm("lg2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// 16 bytes, of which the first `bytes` come from src and the rest are zeros.
 // K and V rows are read once: they may leave L2 before what the kernels after this one read.
 __device__ __forceinline__ uint64_t ReadOncePolicy() {
     uint64_t policy;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(policy));
     return policy;
 }
+// 16 bytes, of which the first `bytes` come from src and the rest are zeros.
 __device__ __forceinline__ void CopyAsync16(uint32_t dst, const void *src, uint32_t bytes, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;\n" ::"r"(dst), "l"(src), "r"(bytes), "l"(policy)
                  : "memory");
@@ -373,7 +378,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
     const uint32_t tiles_at = ring + warp * 2 * Shape::kTileBytes;
     const uint32_t copy_piece = lane % kPieces, copy_row = lane / kPieces;
     const uint32_t copy_to = copy_row * Shape::kRowBytes + ((copy_piece ^ copy_row) * 16);  // of the first copy
-    const int64_t copy_from = static_cast<int64_t>(copy_row) * p.pools.token_stride + (copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? copy_piece * 16 : 0);
+    const int64_t copy_from = static_cast<int64_t>(copy_row) * p.pools.token_stride +
+                              (copy_piece * 8 < static_cast<uint32_t>(p.pools.head_dim) ? copy_piece * 16 : 0);
     // Starts the copies of this warp's tile of the next step; rows that take no part become zeros, so that whatever lies
     // there cannot reach a product.
     auto load_tile = [&](int to_stage) {

@@ -11,8 +11,13 @@
 // thread-block cluster does, each CTA with a slice of the keys in shared memory and the counts added up over distributed
 // shared memory.  That kernel is a chain of short phases, bound by their latencies; it leaves a list of moves.  The
 // second kernel is bound by HBM: it spreads the moves of all heads over the whole GPU, so that one long sequence is
-// packed by every SM.  (One kernel for both left the rows of a head to the cluster that ranked it: 703 us
-// for 131,072 slots of eight heads.)
+// packed by every SM.  (One kernel for both left the rows of a head to the cluster that ranked it: 703 us for 131,072
+// slots of eight heads instead of 78.)
+//
+// 128 heads of 6001 to 8192 slots cut to 4096, rows of 256 bytes: 22 us to rank, 49 us to move (4.9 TB/s read and
+// written, 76 % of a plain copy: 256-byte rows scattered on both sides).  One sequence of 131,072 slots cut to 32,768, all
+// heads together: 37 us and 36 us (88 %).  256 heads one slot over their budget: 14.5 us together, a chain of latencies.
+// Counting with warp-wide matches instead of four copies of the counts took 29 and 61 us to rank the first two.
 #include <cooperative_groups.h>
 
 #include "paged_kv.cuh"

@@ -409,9 +409,9 @@ def test_evict_matches_the_definition(lens, budget, recent, hkv, hw, dim, page, 
 
 
 @pytest.mark.parametrize("in_place", [True, False])
-@pytest.mark.parametrize("tokens", [131072, 500009])
+@pytest.mark.parametrize("tokens", [131072, 360000, 500009])
 def test_evict_one_long_sequence(tokens, in_place):
-    """Over a whole cluster; the longer one does not fit its shared memory."""
+    """Over a whole cluster; the second fills its shared memory, the third does not fit."""
     case = _evict_case(tokens, [tokens], 1, 1, 8, page=64, ties=tokens % 2 == 1, mixed=False)
     _check_evict(*case, tokens // 3, 1000, in_place)
 
