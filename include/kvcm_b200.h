@@ -996,7 +996,8 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
  * (kvcm_b200_attend_workspace_bytes, 16-byte aligned, contents irrelevant); calls that may run at the same time need
  * separate workspaces.  Results do not depend on timing: the same inputs give the same bits.
  * head_dim is a multiple of 8, at most 256; pool addresses and strides are multiples of 16 bytes, query addresses and
- * strides of 4 bytes; at most 65,536 sequences and 2^30 tokens of table per sequence. */
+ * strides of 4 bytes; at most 65,536 sequences, 4,096 query heads and 2^30 tokens of table per sequence, and 10^11
+ * for batch * n_q_heads * (table tokens / 16 + 3). */
 KVCM_API int64_t kvcm_b200_attend_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t n_kv_heads,
                                                   int32_t head_dim, int64_t table_tokens, int32_t with_weights);
 KVCM_API int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_query, int64_t q_batch_stride,

@@ -1002,7 +1002,9 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
         (with_weights && d_weights == d_weights_out && (w_batch_stride != wo_batch_stride || w_head_stride != wo_head_stride))) {
         return KVCM_ER_INVALID_PARAMS;
     }
-    if (batch > 65536 || n_q_heads > 4096 || table_tokens > kMaxTableTokens) return KVCM_EC_OUT_OF_LIMIT;
+    // Steps are counted in 64 bits over the batch and in 32 within a CTA's run.
+    const double most_steps = static_cast<double>(batch) * n_q_heads * (static_cast<double>(table_tokens) / kTile + 1 + kUnitCost);
+    if (batch > 65536 || n_q_heads > 4096 || table_tokens > kMaxTableTokens || most_steps > 1e11) return KVCM_EC_OUT_OF_LIMIT;
     if ((batch > 0 && (d_query == nullptr || (d_block_table == nullptr && table_width > 0) || d_context_lens == nullptr ||
                        d_out == nullptr || d_workspace == nullptr)) ||
         !RowsAre16ByteAligned(*pools) || (reinterpret_cast<uintptr_t>(d_workspace) & 15u) != 0 ||
@@ -1060,10 +1062,6 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.units = p.kv_groups * p.row_tiles;
     p.k_steps = (pools->head_dim + 15) / 16;
     p.v_minus_k = p.pools.v - p.pools.k;
-    // steps are counted in 64 bits over the batch and in 32 within a CTA's run
-    if (static_cast<double>(batch) * p.units * (static_cast<double>(table_tokens) / p.step_tokens + 1 + kUnitCost) >= 1e11) {
-        return KVCM_EC_OUT_OF_LIMIT;
-    }
     // A few steps are done sooner in one CTA than in several whose shares a second kernel joins: a table of
     // kUncutSteps steps or less leaves every unit whole (one sequence of 100 tokens: 5.2 us instead of 7.5 us).
     p.uncut = table_tokens <= kUncutSteps * p.step_tokens;

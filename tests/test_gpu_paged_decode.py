@@ -669,6 +669,7 @@ def test_refusals_on_the_device():
         lambda: batch_append_kv_pages(None, kv, kv, one, one, dk, dv, torch.zeros(33, device=DEV)),  # more than the head
         lambda: batch_append_kv_pages(None, kv[:, :1], kv[:, :1], one, one, dk, dv, inv),
         lambda: batch_append_kv_pages(None, kv, kv, one, one, dk, dv, inv, query_out=q),
+        lambda: batch_append_kv_pages(None, kv, kv, one, one, dk, dk, inv),
         lambda: batch_append_kv_pages(None, kv, kv, one, one, dk[:, :, :1].expand(-1, -1, 2, -1),
                                       dv[:, :, :1].expand(-1, -1, 2, -1), inv),
     ]

@@ -87,7 +87,7 @@ def test_refusals_of_attend():
                dict(pools=_pools(token_stride=132)), dict(pools=_pools(head_dim=60))):
         assert _attend(**kw) == ADDRESS, kw
     assert _attend(pools=_pools(head_dim=264)) == PARAMS
-    for kw in (dict(batch=65537), dict(hq=4098), dict(width=(1 << 26) + 1)):
+    for kw in (dict(batch=65537), dict(hq=4098), dict(width=(1 << 26) + 1), dict(batch=65536, hq=64, width=1 << 20, size=1 << 62)):
         assert _attend(**kw) == LIMIT, kw
 
 
