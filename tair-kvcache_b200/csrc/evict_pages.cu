@@ -73,8 +73,9 @@ struct EvictParams {
 
 template <bool kCluster>
 struct EvictShared {
-    uint32_t merged[kCluster ? kMaxCluster : 1][kBins];  // a pass's counts of every CTA of the cluster
-    uint32_t hist[kPasses][kCopies][kBins + 8];  // one for each pass: peers may still read one pass's while the next counts
+    uint32_t counts[kCluster ? kPasses : 1][kBins];  // of this CTA, the copies added up, for its peers
+    uint32_t total[kBins];                           // of the cluster, in the pass at hand
+    uint32_t hist[kPasses][kCopies][kBins + 8];
     uint2 warp_sum[kEvictWarps];
     uint32_t prefix;  // bytes found so far
     uint32_t wanted;  // keys still to be kept within the prefix
@@ -224,40 +225,28 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             if (kCached && pass == 0 && ages[i] > oldest_safe) keys[i] = key = kKeyProtected;
             if ((key & mask) == prefix) atomicAdd(hist + ((key >> shift) & 0xffu), 1u);
         }
-        sync_all();
-        // Lane t takes the eight bytes 255 - 8 t .. 248 - 8 t, from the top down; the copies of a CTA's counts are added up
-        // by a warp, those of a cluster by a warp each.
-        uint32_t sums[8] = {};
-        if (warp < n_ranks) {
+        __syncthreads();
+        uint32_t counted = 0;  // of byte tid, first in this CTA, then in the cluster
+        if (tid < kBins) {
 #pragma unroll
-            for (int c = 0; c < kCopies; ++c) {
-                const uint4 *from = reinterpret_cast<const uint4 *>(&peer(warp).hist[pass][c][248 - 8 * lane]);
-                const uint4 lo = from[0], hi = from[1];
-                sums[0] += hi.w;
-                sums[1] += hi.z;
-                sums[2] += hi.y;
-                sums[3] += hi.x;
-                sums[4] += lo.w;
-                sums[5] += lo.z;
-                sums[6] += lo.y;
-                sums[7] += lo.x;
-            }
+            for (int c = 0; c < kCopies; ++c) counted += sh.hist[pass][c][tid];
+            if (kCluster) sh.counts[pass][tid] = counted;
         }
         if (kCluster) {
-            if (warp < n_ranks) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sh.merged[warp][j * 32 + lane] = sums[j];
-            }
-            __syncthreads();
-            if (warp == 0) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    sums[j] = 0;
-                    for (uint32_t r = 0; r < n_ranks; ++r) sums[j] += sh.merged[r][j * 32 + lane];
-                }
+            cluster.sync();
+            if (tid < kBins) {
+                counted = 0;
+#pragma unroll 4
+                for (uint32_t r = 0; r < n_ranks; ++r) counted += peer(r).counts[pass][tid];
             }
         }
+        if (tid < kBins) sh.total[tid] = counted;
+        __syncthreads();
         if (warp == 0) {
+            // Lane t takes the eight bytes 255 - 8 t .. 248 - 8 t, from the top down.
+            const uint4 lo = *reinterpret_cast<const uint4 *>(&sh.total[248 - 8 * lane]);
+            const uint4 hi = *reinterpret_cast<const uint4 *>(&sh.total[252 - 8 * lane]);
+            const uint32_t sums[8] = {hi.w, hi.z, hi.y, hi.x, lo.w, lo.z, lo.y, lo.x};
             uint32_t mine = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) mine += sums[j];
@@ -274,10 +263,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
                     const uint32_t byte = 255 - (8 * lane + j);
                     sh.prefix = prefix | (byte << shift);
                     sh.wanted = before + sums[j] == wanted ? kAll : wanted - before;
-                    uint32_t own = 0;  // after the last pass, keys of this CTA that are equal to the threshold
-#pragma unroll
-                    for (int c = 0; c < kCopies; ++c) own += sh.hist[pass][c][byte];
-                    sh.equal = own;
+                    // after the last pass, keys of this CTA that are equal to the threshold
+                    sh.equal = kCluster ? sh.counts[pass][byte] : sums[j];
                 }
                 before += sums[j];
             }
@@ -348,7 +335,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             }
             n_moves += peer(r).movers;
         }
-        cluster.sync();  // a CTA's shared memory may go once its peers have read it
+        cluster.barrier_arrive();  // a CTA's shared memory may go once its peers have read it: they wait at the end
     }
     if (rank == 0 && tid == 0) p.n_moves[unit] = static_cast<int32_t>(n_moves);
     int2 *moves = p.moves + static_cast<int64_t>(unit) * p.max_moves;
@@ -394,6 +381,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) EvictPagesKernel(const __gri
             }
         }
     }
+    if (kCluster) cluster.barrier_wait();
 }
 
 // The moves: rows of K and V in 16-byte pieces, weight and position; the slot a token leaves becomes free.
