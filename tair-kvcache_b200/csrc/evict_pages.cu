@@ -12,12 +12,13 @@
 // shared memory.  That kernel is a chain of short phases, bound by their latencies; it leaves a list of moves.  The
 // second kernel is bound by HBM: it spreads the moves of all heads over the whole GPU, so that one long sequence is
 // packed by every SM.  (One kernel for both left the rows of a head to the cluster that ranked it: 703 us for 131,072
-// slots of eight heads instead of 78.)
+// slots of eight heads instead of 59.)
 //
-// 128 heads of 6001 to 8192 slots cut to 4096, rows of 256 bytes: 22 us to rank, 49 us to move (4.9 TB/s read and
-// written, 76 % of a plain copy: 256-byte rows scattered on both sides).  One sequence of 131,072 slots cut to 32,768, all
-// heads together: 37 us and 36 us (88 %).  256 heads one slot over their budget: 14.5 us together, a chain of latencies.
-// Counting with warp-wide matches instead of four copies of the counts took 29 and 61 us to rank the first two.
+// 128 heads of 6001 to 8192 slots cut to 4096, rows of 256 bytes: 18 us to rank, 45 us to move (5.4 TB/s read and
+// written, 83 % of a plain copy: 256-byte rows scattered on both sides).  One sequence of 131,072 slots cut to 32,768, all
+// heads together: 23 us and 33 us (96 %).  256 heads one slot over their budget: 14 us together, a chain of latencies.
+// Counting with warp-wide matches instead of four copies of the counts took 29 and 61 us to rank the first two; reading
+// all four copies of every peer instead of their sum 22 and 37; moving with plain instead of streaming stores 49 and 36.
 #include <cooperative_groups.h>
 
 #include "paged_kv.cuh"
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_con
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                if (to[u] != nullptr) *reinterpret_cast<uint4 *>(to[u]) = data[u];
+                if (to[u] != nullptr) __stcs(reinterpret_cast<uint4 *>(to[u]), data[u]);
             }
         }
     }
