@@ -276,4 +276,5 @@ def call_pages(name, pools, *args):
     if mod is not None:
         check(getattr(mod, name[len("kvcm_b200_"):])(*pools, *args), name)
         return
-    call(name, ctypes.addressof(KvPools(*pools)), *args)
+    held = KvPools(*pools)  # an address alone would not keep it
+    call(name, ctypes.addressof(held), *args)

@@ -166,3 +166,20 @@ def test_rotary_frequencies():
                 dict(rotary_dim=8, base=1.0), dict(rotary_dim=8, scaling="llama3", high_freq_factor=1.0)):
         with pytest.raises(ValueError):
             rotary_frequencies(device="cpu", **bad)
+
+
+def test_pools_live_until_the_call_without_the_shim(monkeypatch):
+    """Without the shim the entry points get the address of a struct: it has to hold its fields while they run."""
+    fields = (4096, 8192, 10, 20, 30, 40, 16, 2, 64, _cabi.DTYPE_FP16)
+    seen = []
+
+    def fake(name, pools, *args):
+        others = [_cabi.KvPools(*[7] * 10) for _ in range(64)]  # would take the place of one that was freed
+        held = pools if isinstance(pools, _cabi.KvPools) else _cabi.KvPools.from_address(
+            pools if isinstance(pools, int) else ctypes.addressof(pools._obj))
+        seen.append((tuple(getattr(held, f[0]) for f in _cabi.KvPools._fields_), args, len(others)))
+
+    monkeypatch.setattr(_cabi, "shim", lambda: None)
+    monkeypatch.setattr(_cabi, "call", fake)
+    _cabi.call_pages("kvcm_b200_evict_pages", fields, 1, 2)
+    assert seen == [(fields, (1, 2), 64)]
