@@ -990,7 +990,8 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
  * for the attended t; other entries are left as they are.  The two may be the same memory with the same strides.
  * Strides of both, in elements, between sequences and between heads; every row has table_width * page_tokens entries.
  * Scores, softmax statistics, the sums and the weights are held in 32 bits; probabilities enter the product with V as
- * two 16-bit halves, so that only the output is rounded to 16 bits.
+ * two 16-bit halves, so that only the output is rounded to 16 bits: they keep 16 bits in bf16, and in fp16 22 bits down
+ * to 2^-28 of the largest of the head, with an error below 2^-40 of it.
  * The work is cut into equal shares over the GPU's SMs wherever sequences begin and end, so one long sequence uses all
  * of them; shares of one head are joined by a second kernel.  d_workspace holds the shares
  * (kvcm_b200_attend_workspace_bytes, 16-byte aligned, contents irrelevant); calls that may run at the same time need

@@ -14,9 +14,12 @@
 // loading its own tile, the four barrier operations a tile needs, about 100 cycles each, did.)  A group is far too
 // small for the 128 rows of the tcgen05 instructions, and the tensor pipe is idle most of the time as it is.
 //
-// Probabilities enter the second product as two 16-bit halves, p = hi + lo, whose sum carries 16 (bf16) or more bits,
-// so the output is rounded once.  With a group of at most eight the halves cost nothing: hi takes rows 0-7 of the
-// matrix instruction, lo the rows 8-15 that the group leaves free.
+// Probabilities enter the second product as two 16-bit halves, p = hi + lo, whose sum carries 16 (bf16) or 22 (fp16) bits,
+// so the output is rounded once.  fp16 has nothing between 0 and 2^-24, so there the product takes p times 2^15, and the sums
+// are brought back where a share is written: all 22 bits are kept down to 2^-28 of the largest probability and errors
+// stay below 2^-40 of it, where without the factor a token 18 nats below an attention sink was lost whole.  With a group of
+// at most eight the halves cost nothing: hi takes rows 0-7 of the matrix instruction, lo the rows 8-15 that the group
+// leaves free.
 //
 // The work is cut by tokens, not by sequences: the steps (four tiles of one sequence) of the whole batch are numbered
 // through, and each of the persistent CTAs takes an equal run of them, found from the lengths on the device.  Finishing a
@@ -229,9 +232,21 @@ __device__ __forceinline__ void MatrixMultiply<__half>(float (&c)[4], uint32_t a
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// p0, p1 as 16-bit halves: hi is p rounded, lo what the rounding left over, rounded again.
+// What probabilities are multiplied by before they are split, and its inverse.  bf16 has the exponents of a float.
+template <typename T>
+struct SplitScale {
+    static constexpr float kUp = 1.0f, kDown = 1.0f;
+};
+template <>
+struct SplitScale<__half> {
+    static constexpr float kUp = 32768.0f, kDown = 1.0f / 32768.0f;  // the largest stays finite
+};
+
+// p0, p1 as 16-bit halves: hi is p (scaled) rounded, lo what the rounding left over, rounded again.
 template <typename T>
 __device__ __forceinline__ void SplitPair(float p0, float p1, uint32_t &hi, uint32_t &lo) {
+    p0 *= SplitScale<T>::kUp;
+    p1 *= SplitScale<T>::kUp;
     const auto h = Half16<T>::FromFloat2(p0, p1);
     const float2 back = Half16<T>::ToFloat2(h);
     const auto l = Half16<T>::FromFloat2(p0 - back.x, p1 - back.y);
@@ -636,11 +651,12 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<kDim, kScores>::kC
             float *mine_o = reinterpret_cast<float *>(sums + warp * 2 * Shape::kTileBytes) + (lane >> 2) * kDim + (lane & 3) * 2;
 #pragma unroll
             for (int j = 0; j < kOut; ++j) {
+                constexpr float kDown = SplitScale<T>::kDown;
                 if constexpr (kRows == 8) {
-                    *reinterpret_cast<float2 *>(mine_o + j * 8) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+                    *reinterpret_cast<float2 *>(mine_o + j * 8) = make_float2((o[j][0] + o[j][2]) * kDown, (o[j][1] + o[j][3]) * kDown);
                 } else {
-                    *reinterpret_cast<float2 *>(mine_o + j * 8) = make_float2(o[j][0], o[j][1]);
-                    *reinterpret_cast<float2 *>(mine_o + 8 * kDim + j * 8) = make_float2(o[j][2], o[j][3]);
+                    *reinterpret_cast<float2 *>(mine_o + j * 8) = make_float2(o[j][0] * kDown, o[j][1] * kDown);
+                    *reinterpret_cast<float2 *>(mine_o + 8 * kDim + j * 8) = make_float2(o[j][2] * kDown, o[j][3] * kDown);
                 }
             }
             __syncthreads();
