@@ -935,28 +935,38 @@ AttendWorkspace LayOut(int32_t batch, int32_t n_q_heads, int32_t group, int32_t 
 }
 
 template <typename T, int kDim, int kRows, bool kScores>
-void LaunchAttend(AttendParams p, cudaStream_t stream) {
+int32_t LaunchAttend(AttendParams p, cudaStream_t stream) {
     using Shape = AttendShape<kDim, kScores>;
     static_assert((Shape::kRingBytes + 2048) * Shape::kCtasPerSm <= 228 * 1024, "CTAs per SM");
     auto *main_kernel = AttendPagesKernel<T, kDim, kRows, kScores>;
-    EnsureDynamicSmem(main_kernel, Shape::kRingBytes);
     const int32_t sm_count = GetDeviceInfo().sm_count;
     p.copy_stride = (32 / (kDim / 8)) * p.pools.token_stride;
     p.workers = std::min(kMaxWorkers, sm_count * Shape::kCtasPerSm);
-    main_kernel<<<p.uncut ? p.batch * p.units : p.workers, kAttendThreads, Shape::kRingBytes, stream>>>(p);
+    Requests requests;
+    requests.Make([&] { return EnsureDynamicSmem(main_kernel, Shape::kRingBytes); });
+    requests.Make([&] {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<uint32_t>(p.uncut ? p.batch * p.units : p.workers));
+        cfg.blockDim = dim3(kAttendThreads);
+        cfg.dynamicSmemBytes = Shape::kRingBytes;
+        cfg.stream = stream;
+        return cudaLaunchKernelEx(&cfg, main_kernel, p);
+    });
 
     // The kernels that follow wait on the device for the one before them; their launch overlaps it.
     auto launch_after = [&](auto kernel, int32_t blocks) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(static_cast<uint32_t>(blocks));
-        cfg.blockDim = dim3(kJoinThreads);
-        cfg.stream = stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, kernel, p);
+        requests.Make([&] {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(static_cast<uint32_t>(blocks));
+            cfg.blockDim = dim3(kJoinThreads);
+            cfg.stream = stream;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            return cudaLaunchKernelEx(&cfg, kernel, p);
+        });
     };
     if (!p.uncut) launch_after(JoinSharesKernel<T, kDim, kRows, kScores>, p.workers);
     if (kScores) {
@@ -964,26 +974,22 @@ void LaunchAttend(AttendParams p, cudaStream_t stream) {
         const bool many_heads = p.n_weight_heads == 1 && p.n_q_heads >= 8;
         launch_after(many_heads ? AddWeightsKernel<kJoinThreads, 1, 8> : AddWeightsKernel<kJoinThreads, 4, 4>, 8 * sm_count);
     }
+    return requests.Status();
 }
 
 template <typename T, int kDim>
-void DispatchAttend(const AttendParams &p, cudaStream_t stream) {
+int32_t DispatchAttend(const AttendParams &p, cudaStream_t stream) {
     if (p.group <= 8) {
-        p.scores != nullptr ? LaunchAttend<T, kDim, 8, true>(p, stream) : LaunchAttend<T, kDim, 8, false>(p, stream);
-    } else {
-        p.scores != nullptr ? LaunchAttend<T, kDim, 16, true>(p, stream) : LaunchAttend<T, kDim, 16, false>(p, stream);
+        return p.scores != nullptr ? LaunchAttend<T, kDim, 8, true>(p, stream) : LaunchAttend<T, kDim, 8, false>(p, stream);
     }
+    return p.scores != nullptr ? LaunchAttend<T, kDim, 16, true>(p, stream) : LaunchAttend<T, kDim, 16, false>(p, stream);
 }
 
 template <typename T>
-void DispatchAttend(const AttendParams &p, cudaStream_t stream) {
-    if (p.pools.head_dim <= 64) {
-        DispatchAttend<T, 64>(p, stream);
-    } else if (p.pools.head_dim <= 128) {
-        DispatchAttend<T, 128>(p, stream);
-    } else {
-        DispatchAttend<T, 256>(p, stream);
-    }
+int32_t DispatchAttend(const AttendParams &p, cudaStream_t stream) {
+    if (p.pools.head_dim <= 64) return DispatchAttend<T, 64>(p, stream);
+    if (p.pools.head_dim <= 128) return DispatchAttend<T, 128>(p, stream);
+    return DispatchAttend<T, 256>(p, stream);
 }
 
 }  // namespace
@@ -1089,12 +1095,8 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     for (int32_t i = 0; i < 31; ++i) {
         if (pools->page_tokens == 1 << i) p.page_shift = i;
     }
-    if (pools->dtype == KVCM_DTYPE_BF16) {
-        DispatchAttend<__nv_bfloat16>(p, AsStream(stream));
-    } else {
-        DispatchAttend<__half>(p, AsStream(stream));
-    }
-    return LaunchStatus();
+    return pools->dtype == KVCM_DTYPE_BF16 ? DispatchAttend<__nv_bfloat16>(p, AsStream(stream))
+                                           : DispatchAttend<__half>(p, AsStream(stream));
 }
 
 }  // extern "C"

@@ -33,7 +33,8 @@ constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 256;
 constexpr int kPasses = 4;
 constexpr int kCopies = 4;  // of the counts, for lanes that count the same byte: weights share their high ones
-constexpr int kMaxCluster = 16;  // beyond 8 a launch opts in
+constexpr int kMaxCluster = 16;
+constexpr int kPortableCluster = 8;  // beyond it a launch opts in
 constexpr uint32_t kKeyProtected = 0xFFFFFFFFu;
 constexpr uint32_t kKeyNan = 0xFFFFFFFEu;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
@@ -458,8 +459,40 @@ __global__ void __launch_bounds__(kMoveThreads) MoveSlotsKernel(const __grid_con
 
 // The opt-in to clusters of more than eight CTAs is per device and per kernel, like the one to large shared memory.
 template <typename Kernel>
-void AllowLargeClusters(Kernel kernel) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+cudaError_t AllowLargeClusters(Kernel kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+
+// The largest cluster to launch: sixteen CTAs, each with an SM's shared memory, where the device (or the partition of it
+// that the process has) can place that many side by side, else the eight that any can.  Asked once per device.
+int LargestCluster() {
+    static std::mutex mu;
+    static std::vector<std::pair<int, int>> known;  // by device ordinal
+    int device = 0;
+    cudaGetDevice(&device);
+    std::lock_guard<std::mutex> lock(mu);
+    for (const auto &k : known) {
+        if (k.first == device) return k.second;
+    }
+    auto *kernel = EvictPagesKernel<true, true>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kMaxCluster);
+    cfg.blockDim = dim3(kEvictThreads);
+    cfg.dynamicSmemBytes = kMaxCachedSlots * 8;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kMaxCluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const bool placed = EnsureDynamicSmem(kernel, kMaxCachedSlots * 8) == cudaSuccess &&
+                        AllowLargeClusters(kernel) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+    if (!placed) cudaGetLastError();
+    known.emplace_back(device, placed ? kMaxCluster : kPortableCluster);
+    return known.back().second;
 }
 
 int64_t EvictMaxMoves(int64_t table_tokens, int32_t budget) {
@@ -553,9 +586,10 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     // As many CTAs as fit two to an SM, but none with fewer than about a thousand slots, and slices that fit shared memory.
     const int64_t units = static_cast<int64_t>(batch) * n_weight_heads;
     const int32_t sm_count = GetDeviceInfo().sm_count;
+    const int largest = LargestCluster();
     int cluster = 1;
-    while (cluster < kMaxCluster && units * cluster * 2 <= 2 * sm_count && table_tokens / (cluster * 2) >= 1024) cluster *= 2;
-    while (cluster < kMaxCluster && (table_tokens + cluster - 1) / cluster > kMaxCachedSlots) cluster *= 2;
+    while (cluster < largest && units * cluster * 2 <= 2 * sm_count && table_tokens / (cluster * 2) >= 1024) cluster *= 2;
+    while (cluster < largest && (table_tokens + cluster - 1) / cluster > kMaxCachedSlots) cluster *= 2;
     const int64_t slice = (table_tokens + cluster - 1) / cluster;
     const bool cached = slice <= kMaxCachedSlots;
     p.units = static_cast<int32_t>(units);
@@ -575,17 +609,18 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
+    Requests requests;
     auto launch = [&](auto kernel) {
-        if (cached) EnsureDynamicSmem(kernel, kMaxCachedSlots * 8);
-        if (cluster > 8) AllowLargeClusters(kernel);
-        cudaLaunchKernelEx(&cfg, kernel, p);
+        if (cached) requests.Make([&] { return EnsureDynamicSmem(kernel, kMaxCachedSlots * 8); });
+        if (cluster > kPortableCluster) requests.Make([&] { return AllowLargeClusters(kernel); });
+        requests.Make([&] { return cudaLaunchKernelEx(&cfg, kernel, p); });
     };
     if (cluster > 1) {
         cached ? launch(EvictPagesKernel<true, true>) : launch(EvictPagesKernel<true, false>);
     } else {
         launch(EvictPagesKernel<false, true>);  // a slice too long for shared memory has made a cluster above
     }
-    if (p.blocks_per_unit == 0) return LaunchStatus();  // the budget is not below what the table holds
+    if (p.blocks_per_unit == 0) return requests.Status();  // the budget is not below what the table holds
     cudaLaunchConfig_t move = {};
     move.gridDim = dim3(static_cast<uint32_t>(std::min<int64_t>(units * p.blocks_per_unit, 8 * sm_count)));
     move.blockDim = dim3(kMoveThreads);
@@ -595,8 +630,8 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     early[0].val.programmaticStreamSerializationAllowed = 1;
     move.attrs = early;
     move.numAttrs = 1;
-    cudaLaunchKernelEx(&move, MoveSlotsKernel, p);
-    return LaunchStatus();
+    requests.Make([&] { return cudaLaunchKernelEx(&move, MoveSlotsKernel, p); });
+    return requests.Status();
 }
 
 }  // extern "C"

@@ -38,7 +38,7 @@ bool HaveDevice();
 // The opt-in to more than 48 KiB of dynamic shared memory is per device and per kernel; this makes it
 // once for each pair, whichever host thread gets there first.
 template <typename Kernel>
-inline void EnsureDynamicSmem(Kernel kernel, int bytes) {
+inline cudaError_t EnsureDynamicSmem(Kernel kernel, int bytes) {
     static std::mutex mu;
     static std::vector<std::pair<int, const void *>> done;
     int device = 0;
@@ -46,9 +46,11 @@ inline void EnsureDynamicSmem(Kernel kernel, int bytes) {
     const std::pair<int, const void *> key(device, reinterpret_cast<const void *>(kernel));
     std::lock_guard<std::mutex> lock(mu);
     if (std::find(done.begin(), done.end(), key) == done.end()) {
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (error != cudaSuccess) return error;
         done.push_back(key);
     }
+    return cudaSuccess;
 }
 
 __device__ __forceinline__ uint32_t LaneId() { return threadIdx.x & 31u; }

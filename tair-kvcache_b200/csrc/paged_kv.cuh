@@ -56,6 +56,24 @@ inline bool RowsAre16ByteAligned(const kvcm_b200_kv_pools_t &p) {
            ((p.page_stride | p.token_stride | p.head_stride | p.head_dim) & 7) == 0;
 }
 
+// What a call asks of the CUDA runtime, in order, and nothing after the first request that is refused: the kernels that
+// follow another take their work from the workspace, and without it would run on whatever lies there.
+class Requests {
+public:
+    template <typename Request>
+    void Make(Request request) {
+        if (error_ == cudaSuccess) error_ = request();
+    }
+    int32_t Status() const {
+        if (error_ == cudaSuccess) return LaunchStatus();
+        cudaGetLastError();  // what is reported here is not reported again
+        return KVCM_ER_CUDAMEMCPY_ERROR;
+    }
+
+private:
+    cudaError_t error_ = cudaSuccess;
+};
+
 // n / d for 32-bit numbers by one wide multiplication: magic = floor(2^64 / d) + 1 (0 for d = 1) is exact for all of them.
 struct FastDivide {
     uint64_t magic;
