@@ -21,6 +21,8 @@
 // all four copies of every peer instead of their sum 22 and 37; moving with plain instead of streaming stores 49 and 36.
 #include <cooperative_groups.h>
 
+#include <cstddef>
+
 #include "paged_kv.cuh"
 
 namespace cg = cooperative_groups;
@@ -74,9 +76,9 @@ struct EvictParams {
 };
 
 template <bool kCluster>
-struct EvictShared {
+struct alignas(16) EvictShared {
     uint32_t counts[kCluster ? kPasses : 1][kBins];  // of this CTA, the copies added up, for its peers
-    uint32_t total[kBins];                           // of the cluster, in the pass at hand
+    uint32_t total[kBins];                           // of the cluster, in the pass at hand; read 16 bytes at a time
     uint32_t hist[kPasses][kCopies][kBins + 8];
     uint2 warp_sum[kEvictWarps];
     uint32_t prefix;  // bytes found so far
@@ -86,6 +88,8 @@ struct EvictShared {
     uint32_t movers;  // this CTA's movers
     int32_t newest;
 };
+static_assert(alignof(EvictShared<true>) == 16 && offsetof(EvictShared<true>, total) % 16 == 0, "total is read as uint4");
+static_assert(alignof(EvictShared<false>) == 16 && offsetof(EvictShared<false>, total) % 16 == 0, "total is read as uint4");
 
 // Unsigned order of the result = order of the weights; both zeros are equal, NaN is the largest.
 __device__ __forceinline__ uint32_t WeightKey(float w) {
