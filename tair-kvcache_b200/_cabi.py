@@ -269,6 +269,9 @@ def call_move(name, *args):
     call(name, *args)
 
 
+_WIDTHS = {_i32: 32, _i64: 64}
+
+
 def call_pages(name, pools, *args):
     """A decode-step entry point by its C name; `pools` holds the fields of kvcm_b200_kv_pools_t in order and addresses
     are integers (0 = NULL).  Through the pybind shim when it is built, else through ctypes."""
@@ -276,5 +279,8 @@ def call_pages(name, pools, *args):
     if mod is not None:
         check(getattr(mod, name[len("kvcm_b200_"):])(*pools, *args), name)
         return
+    for value, ctype in zip((*pools[2:], *args), (*[f[1] for f in KvPools._fields_[2:]], *SIGNATURES[name][1:])):
+        if ctype in _WIDTHS and not -1 << _WIDTHS[ctype] - 1 <= value < 1 << _WIDTHS[ctype] - 1:
+            raise TypeError("%s: %d does not fit %d bits" % (name, value, _WIDTHS[ctype]))  # ctypes would cut it
     held = KvPools(*pools)  # an address alone would not keep it
     call(name, ctypes.addressof(held), *args)

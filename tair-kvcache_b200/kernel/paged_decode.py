@@ -277,6 +277,7 @@ def _attend_plan(window, out, lse, weights, weights_out, *flat):
     if lse is not None and (lse[0] != query[0][:2] or lse[2] != torch.float32 or lse[3] != k[3] or not _contiguous(lse)):
         raise ValueError("lse must be a contiguous float32 [sequences, q_heads] tensor on the pools' device")
     tokens = width * pools[4]
+    window = min(window, max(tokens, 1)) if window else 0  # one beyond the table is none, and 32 bits hold this
     w_args = wo_args = None
     if weights is not None:
         w_args = _per_slot(weights, "weights", torch.float32, k, batch, tokens)
@@ -286,7 +287,7 @@ def _attend_plan(window, out, lse, weights, weights_out, *flat):
         raise ValueError("weights_out without weights")
     size = _workspace_bytes("kvcm_b200_attend_pages", _cabi.lib().kvcm_b200_attend_workspace_bytes(
         batch, n_q_heads, n_kv_heads, dim, tokens, int(weights is not None)))
-    return pools, (*q_args[:2], batch, n_q_heads), (table_stride, width), w_args, wo_args, size, dim ** -0.5, k[3]
+    return pools, (*q_args[:2], batch, n_q_heads), (table_stride, width), window, w_args, wo_args, size, dim ** -0.5, k[3]
 
 
 def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -307,7 +308,7 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     the attention each token got, summed over the query heads of its KV head or, with one weight head, over all of
     them - what batch_evict_kv_pages ranks by.  Entries that are not attended are left as they are."""
     _no_grad(query, k_pool, v_pool, weights)
-    pools, q_args, table_args, w_args, wo_args, size, default_scale, device = _attend_plan(
+    pools, q_args, table_args, window, w_args, wo_args, size, default_scale, device = _attend_plan(
         int(window), out if out is None else _layout(out), lse if lse is None else _layout(lse),
         weights if weights is None else _layout(weights), weights_out if weights_out is None else _layout(weights_out),
         query.shape, query.stride(), query.dtype, query.device, k_pool.shape, k_pool.stride(), k_pool.dtype, k_pool.device,
@@ -321,7 +322,7 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
     _launch("kvcm_b200_attend_pages", device, (k_pool.data_ptr(), v_pool.data_ptr(), *pools), query.data_ptr(), *q_args,
             block_table.data_ptr(), *table_args, context_lens.data_ptr(), default_scale if scale is None else float(scale),
-            int(window), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *w_all, workspace.data_ptr(), size,
+            window, out.data_ptr(), 0 if lse is None else lse.data_ptr(), *w_all, workspace.data_ptr(), size,
             _status_ptr(status, device))
     return out
 

@@ -7,6 +7,7 @@ import torch
 import paged_decode_oracle as oracle
 from test_gpu_paged_decode import DEV, _attend_case, _attend_tolerance
 
+from tair_kvcache_b200 import _cabi
 from tair_kvcache_b200.kernel import batch_attend_kv_pages
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +38,13 @@ def test_attend_with_a_sink_whose_value_is_zero(dtype, nats, hq, hkv, window):
     off = (got.cpu().double() - want).abs()
     assert (off <= tol).all(), ((off / tol).max(), (off / want.abs()).max())
     assert (want.abs() > 0).all() and math.isfinite(tol.max())
+
+
+@pytest.mark.parametrize("shim", [True, False])
+def test_attend_with_a_window_beyond_32_bits(shim, monkeypatch):
+    if not shim:
+        monkeypatch.setattr(_cabi, "shim", lambda: None)
+    q, k_pool, v_pool, table, lens = (t.to(DEV) for t in _attend_case(31, [700, 30], 8, 2, 64, "bf16"))
+    want = batch_attend_kv_pages(q, k_pool, v_pool, table, lens)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63):
+        assert torch.equal(batch_attend_kv_pages(q, k_pool, v_pool, table, lens, window=window), want), window

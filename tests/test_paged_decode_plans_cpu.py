@@ -1,0 +1,62 @@
+"""What the Python operators hand to the entry points, from layouts alone: no GPU is needed to describe a tensor on one."""
+import math
+
+import pytest
+import torch
+
+import tair_kvcache_b200  # noqa: F401
+from tair_kvcache_b200 import _cabi
+from tair_kvcache_b200.kernel import paged_decode
+
+GPU = torch.device("cuda", 0)
+
+
+def contiguous(shape):
+    return tuple(math.prod(shape[i + 1:]) for i in range(len(shape)))
+
+
+def layout(shape, dtype, stride=None):
+    return torch.Size(shape), contiguous(shape) if stride is None else stride, dtype, GPU
+
+
+def flat(*layouts):
+    return [field for one in layouts for field in one]
+
+
+POOL = layout((10, 16, 2, 64), torch.bfloat16)
+QUERY = layout((3, 4, 64), torch.bfloat16)
+TABLE = layout((3, 5), torch.int32)
+LENS = layout((3,), torch.int32)
+
+
+def attend_plan(window=0, out=None, lse=None, weights=None, weights_out=None, query=QUERY, k=POOL, v=POOL, table=TABLE, lens=LENS):
+    return paged_decode._attend_plan(window, out, lse, weights, weights_out, *flat(query, k, v, table, lens))
+
+
+def test_a_window_beyond_the_table_is_the_table():
+    for window, handed in ((0, 0), (1, 1), (79, 79), (80, 80), (81, 80), (2 ** 31, 80), (2 ** 32, 80), (2 ** 32 + 5, 80), (2 ** 70, 80)):
+        assert attend_plan(window)[3] == handed, window
+    assert attend_plan(7, table=layout((3, 0), torch.int32))[3] == 1  # no window would be another call
+    with pytest.raises(ValueError):
+        attend_plan(-1)
+
+
+def test_integers_are_not_cut_without_the_shim(monkeypatch):
+    """ctypes would pass 2^32 + 5 on as 5; the shim refuses it, and so does the route without it."""
+    monkeypatch.setattr(_cabi, "shim", lambda: None)
+    called = []
+    monkeypatch.setattr(_cabi, "call", lambda name, *args: called.append(args))
+    pools = (4096, 8192, 10, 2048, 128, 64, 16, 2, 64, 0)
+    args = [0, 0, 0, 0, 0, 0, 0, 4096, 128, 64, 4096, 128, 64, 4096, 8, 4096, 4, 3, 4096, 64, 0, 1.0, 0, 0]
+    _cabi.call_pages("kvcm_b200_append_pages", pools, *args)
+    assert len(called) == 1 and called[0][1:] == tuple(args)
+    tokens = 17
+    assert _cabi.SIGNATURES["kvcm_b200_append_pages"][1:][tokens] is _cabi._i32 and args[tokens] == 3
+    for value in (2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1):
+        with pytest.raises(TypeError):
+            _cabi.call_pages("kvcm_b200_append_pages", pools, *args[:tokens], value, *args[tokens + 1:])
+    with pytest.raises(TypeError):  # page_tokens
+        _cabi.call_pages("kvcm_b200_append_pages", (*pools[:6], 2 ** 32 + 16, *pools[7:]), *args)
+    with pytest.raises(TypeError):  # a stride
+        _cabi.call_pages("kvcm_b200_append_pages", (*pools[:3], 2 ** 63, *pools[4:]), *args)
+    assert len(called) == 1
