@@ -10,8 +10,8 @@ on them to the engine; slot and page numbers mean here what they mean there.  A 
 indexed [page, token, head, element] - any strides of the first three, so both [pages, page_tokens, heads, dim] tensors
 and .transpose(1, 2) views of [pages, heads, page_tokens, dim] ones.  The calls return as soon as the kernels are
 enqueued on the current stream of the pools' device and allocate nothing but their results and workspaces, from torch's
-allocator, so they can be captured into a CUDA graph.  None of them is differentiable; inputs that require gradients
-are refused while gradients are recorded.
+allocator, so they can be captured into a CUDA graph.  None of them is differentiable; tensors that require
+gradients, read or written, are refused while gradients are recorded.
 """
 import functools
 import math
@@ -237,7 +237,7 @@ def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, valu
     page * page_tokens + offset, the numbers batch_scatter_kv_caches takes; -1 marks a padding token, which writes
     nothing; any other slot outside the pool is skipped and counted in `status` (four zeroed 32-bit words on the GPU).
     The same slot twice in one call is a data race.  `query_out` may be `query`."""
-    _no_grad(query, key, value, inv_freq, k_pool, v_pool)
+    _no_grad(query, key, value, inv_freq, k_pool, v_pool, query_out)
     if not isinstance(slot_indices, torch.Tensor):
         slot_indices = _index_tensor(slot_indices, k_pool.device)
     pools, tokens, q_args, q_out_args, k_args, v_args, position_bytes, slot_bytes, rotary_dim, device = _append_plan(
@@ -307,7 +307,7 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself) receives weights plus
     the attention each token got, summed over the query heads of its KV head or, with one weight head, over all of
     them - what batch_evict_kv_pages ranks by.  Entries that are not attended are left as they are."""
-    _no_grad(query, k_pool, v_pool, weights)
+    _no_grad(query, k_pool, v_pool, weights, out, lse, weights_out)
     pools, q_args, table_args, window, w_args, wo_args, size, default_scale, device = _attend_plan(
         int(window), out if out is None else _layout(out), lse if lse is None else _layout(lse),
         weights if weights is None else _layout(weights), weights_out if weights_out is None else _layout(weights_out),
@@ -367,7 +367,7 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
 
     Pages are packed in place: a page that two sequences share must be copied first.  A move from or to a page outside
     the pool is left out and counted in `status`, as is a length beyond the table (cut to it)."""
-    _no_grad(k_pool, v_pool, weights)
+    _no_grad(k_pool, v_pool, weights, weights_out)
     pools, table_args, batch, sizes, w_args, p_args, wo_args, po_args, size, device = _evict_plan(
         int(budget), int(recent), weights_out if weights_out is None else _layout(weights_out),
         positions_out if positions_out is None else _layout(positions_out), k_pool.shape, k_pool.stride(), k_pool.dtype,

@@ -60,3 +60,28 @@ def test_integers_are_not_cut_without_the_shim(monkeypatch):
     with pytest.raises(TypeError):  # a stride
         _cabi.call_pages("kvcm_b200_append_pages", (*pools[:3], 2 ** 63, *pools[4:]), *args)
     assert len(called) == 1
+
+
+def test_no_tensor_that_requires_gradients_is_read_or_written():
+    def x(*shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype)
+
+    pools = dict(k_pool=x(4, 16, 2, 64), v_pool=x(4, 16, 2, 64))
+    sequences = dict(block_table=x(1, 2, dtype=torch.int32), context_lens=x(1, dtype=torch.int32))
+    append = dict(query=x(1, 4, 64), key=x(1, 2, 64), value=x(1, 2, 64), positions=x(1, dtype=torch.int64),
+                  slot_indices=x(1, dtype=torch.int64), inv_freq=x(32, dtype=torch.float32), query_out=x(1, 4, 64), **pools)
+    attend = dict(query=x(1, 4, 64), out=x(1, 4, 64), lse=x(1, 4, dtype=torch.float32), weights=x(1, 2, 32, dtype=torch.float32),
+                  weights_out=x(1, 2, 32, dtype=torch.float32), **pools, **sequences)
+    evict = dict(weights=x(1, 2, 32, dtype=torch.float32), positions=x(1, 2, 32, dtype=torch.int32), budget=4,
+                 weights_out=x(1, 2, 32, dtype=torch.float32), **pools, **sequences)
+    for op, kwargs in ((paged_decode.batch_append_kv_pages, append), (paged_decode.batch_attend_kv_pages, attend),
+                       (paged_decode.batch_evict_kv_pages, evict)):
+        for name, t in kwargs.items():
+            if not isinstance(t, torch.Tensor) or not t.is_floating_point():
+                continue
+            t.requires_grad_()
+            with pytest.raises(ValueError, match="no gradient"):
+                op(**kwargs)
+            with torch.no_grad(), pytest.raises(ValueError, match="one GPU"):  # these tensors are on none
+                op(**kwargs)
+            t.requires_grad_(False)
