@@ -84,10 +84,16 @@ def _layouts(flat):
     return [flat[i:i + 4] for i in range(0, len(flat), 4)]
 
 
+def _strides(t):
+    """A layout's strides; that of an axis of length one says nothing and counts as zero."""
+    return tuple(stride if size > 1 else 0 for size, stride in zip(t[0], t[1]))
+
+
 def _pools(k, v):
     """The fields of kvcm_b200_kv_pools_t behind the two addresses, from the pools' layouts."""
-    (shape, strides, dtype, device) = k
-    if len(shape) != 4 or v[0] != shape or v[1] != strides:
+    (shape, _, dtype, device) = k
+    strides = _strides(k)
+    if len(shape) != 4 or v[0] != shape or _strides(v) != strides:
         raise ValueError("the K and V pools must be [pages, page_tokens, heads, dim] tensors of one shape and layout")
     if dtype not in _DTYPES or v[2] != dtype:
         raise ValueError("the pools must hold bfloat16 or float16, got %s and %s" % (dtype, v[2]))
@@ -99,8 +105,6 @@ def _pools(k, v):
         raise ValueError("the pools' pages are empty")
     if se != 1 and dim > 1:
         raise ValueError("the elements of a head must be contiguous in the pools")
-    # the stride of an axis of length one says nothing
-    sp, st, sh = sp if pages > 1 else 0, st if page_tokens > 1 else 0, sh if heads > 1 else 0
     if (pages > 1 and sp == 0) or (page_tokens > 1 and st == 0) or (heads > 1 and sh == 0):
         raise ValueError("rows of the pools share memory")
     return (pages, sp, st, sh, page_tokens, heads, dim, _DTYPES[dtype])
@@ -115,7 +119,7 @@ def _no_grad(*tensors):
 
 def _heads(t, name: str, pool, count: int):
     """A layout of [count, heads, dim] beside a pool's; the strides between tokens and heads, and the number of heads."""
-    shape, strides, dtype, device = t
+    shape, strides, dtype, device = t[0], _strides(t), t[2], t[3]
     if len(shape) != 3 or shape[0] != count or shape[2] != pool[0][3]:
         raise ValueError("%s must be [%d, heads, %d], got %s" % (name, count, pool[0][3], list(shape)))
     if dtype != pool[2] or device != pool[3]:

@@ -8,7 +8,7 @@ import paged_decode_oracle as oracle
 from test_gpu_paged_decode import DEV, _attend_case, _attend_tolerance
 
 from tair_kvcache_b200 import _cabi
-from tair_kvcache_b200.kernel import batch_attend_kv_pages
+from tair_kvcache_b200.kernel import batch_append_kv_pages, batch_attend_kv_pages, rotary_frequencies
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,23 @@ def test_attend_with_a_window_beyond_32_bits(shim, monkeypatch):
     want = batch_attend_kv_pages(q, k_pool, v_pool, table, lens)
     for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63):
         assert torch.equal(batch_attend_kv_pages(q, k_pool, v_pool, table, lens, window=window), want), window
+
+
+def test_one_token_views_with_odd_strides():
+    """The stride of an axis of length one may be anything; these are no multiple of the four bytes a query is read by."""
+    dim, hq, hkv = 64, 4, 2
+    q, k_pool, v_pool, table, lens = (t.to(DEV) for t in _attend_case(5, [90], hq, hkv, dim, "bf16"))
+    want = batch_attend_kv_pages(q, k_pool, v_pool, table, lens)
+    odd = torch.empty(hq * dim + 1, dtype=torch.bfloat16, device=DEV)[:hq * dim].as_strided((1, hq, dim), (hq * dim + 1, dim, 1))
+    odd.copy_(q)
+    assert torch.equal(batch_attend_kv_pages(odd, k_pool, v_pool, table, lens), want)
+    kv = torch.randn(1, hkv, dim, device=DEV).to(torch.bfloat16)
+    odd_kv = torch.empty(hkv * dim, dtype=torch.bfloat16, device=DEV).as_strided((1, hkv, dim), (7, dim, 1))
+    odd_kv.copy_(kv)
+    slot, position = torch.tensor([20], device=DEV), torch.tensor([89], device=DEV)
+    inv_freq, _ = rotary_frequencies(dim, device=DEV)
+    results = []
+    for query, key in ((q, kv), (odd, odd_kv)):
+        pools = torch.zeros_like(k_pool), torch.zeros_like(v_pool)
+        results.append((batch_append_kv_pages(query, key, key, position, slot, *pools, inv_freq), *pools))
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -85,3 +85,27 @@ def test_no_tensor_that_requires_gradients_is_read_or_written():
             with torch.no_grad(), pytest.raises(ValueError, match="one GPU"):  # these tensors are on none
                 op(**kwargs)
             t.requires_grad_(False)
+
+
+def append_plan(query=layout((1, 4, 64), torch.bfloat16), query_out=None, key=layout((1, 2, 64), torch.bfloat16),
+                value=layout((1, 2, 64), torch.bfloat16), k=POOL, v=POOL):
+    index = layout((key[0][0],), torch.int64)
+    return paged_decode._append_plan(query, query_out, *flat(key, value, index, index, k, v, layout((32,), torch.float32)))
+
+
+def test_strides_of_axes_of_length_one_say_nothing():
+    # a view of one token, or of one head, may have any stride there: neither its value nor its alignment counts
+    odd = layout((1, 4, 64), torch.bfloat16, (257, 64, 1))
+    assert attend_plan(query=odd, table=layout((1, 5), torch.int32), lens=layout((1,), torch.int32))[1][:2] == (0, 64)
+    head = layout((3, 2, 64), torch.bfloat16, (128, 64, 1))
+    assert attend_plan(query=head)[1][:2] == (128, 64)
+    one_head = layout((3, 1, 64), torch.bfloat16, (256, 13, 1))
+    pool = layout((10, 16, 1, 64), torch.bfloat16)
+    assert attend_plan(query=one_head, k=pool, v=pool)[1][:2] == (256, 0)
+    plan = append_plan(odd, odd, layout((1, 2, 64), torch.bfloat16, (3, 64, 1)), layout((1, 2, 64), torch.bfloat16, (5, 64, 1)))
+    assert plan[2][:2] == plan[3] == (0, 64) and plan[4] == plan[5] == (0, 64)
+    # pools that differ in such a stride alone have one layout
+    k, v = layout((1, 16, 2, 64), torch.bfloat16, (4096, 128, 64, 1)), layout((1, 16, 2, 64), torch.bfloat16, (9999, 128, 64, 1))
+    assert attend_plan(k=k, v=v)[0][:4] == (1, 0, 128, 64)
+    with pytest.raises(ValueError, match="one shape"):
+        attend_plan(k=POOL, v=layout((10, 16, 2, 64), torch.bfloat16, (4096, 128, 64, 1)))
