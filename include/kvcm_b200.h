@@ -975,9 +975,11 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
                                         int32_t interleaved, float attention_factor, uint32_t *d_status,
                                         kvcm_stream_t stream);
 
-/* Attention of one new token per sequence over its paged keys and values.  Sequence b attends tokens
- * [max(0, len - window), len), len = context_lens[b] (window 0 = all of them); token t lies in page
- * block_table[b * table_stride + t / page_tokens].  Query head h reads KV head h / (n_q_heads / n_kv_heads):
+/* Attention of one new token per sequence over its paged keys and values.  Sequence b attends the tokens in slots
+ * [max(0, len - window), len), len = context_lens[b] (window 0 = all of them); slot t lies in page
+ * block_table[b * table_stride + t / page_tokens].  A window goes by slots: it is the last tokens only while the cache is
+ * in order, until kvcm_b200_evict_pages first moves one.  After that, window = 0; a layer that looks back W tokens keeps
+ * them with budget = recent = W, evicting between append and attention.  Query head h reads KV head h / (n_q_heads / n_kv_heads):
  *   out[b][h] = sum_t p_t V[t],  p = softmax(scale * query[b][h] . K[t])
  * out is [batch][n_q_heads][head_dim] contiguous, of the pools' type; d_lse, when not NULL, receives the natural
  * logarithm of the softmax sum, [batch][n_q_heads].  A sequence without tokens, and a head whose scores are all
@@ -1016,8 +1018,8 @@ KVCM_API int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const
  * whose position is greater than (largest position in use) - recent; then by weight, larger first (NaN counts as the
  * largest); among equals the lower slot.  Survivors that lie below `budget` stay where they are; those above move, in
  * ascending order, into the freed slots below, in ascending order: K row, V row, weight and position (of KV head w, or
- * of all heads when n_weight_heads = 1).  Attention does not depend on the order of slots, and the positions array
- * keeps every token's age.  Slots [budget, len) get weight 0 and position -1; slots from len on are left as they are.
+ * of all heads when n_weight_heads = 1).  Attention without a window does not depend on the order of slots, and
+ * the positions array keeps every token's age.  Slots [budget, len) get weight 0 and position -1; slots from len on are left as they are.
  * new_lens[b] = min(len, budget).  Sequences with len <= budget keep everything.
  * weights_out / positions_out may be the input arrays with the same strides (the usual call) or other memory, which
  * then receives all slots below len; new_lens may not overlap context_lens.  Pages named by the kept part of two sequences at once (a shared prefix) would be

@@ -302,8 +302,10 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     """Attention of one new token per sequence over its cached keys and values; returns [sequences, q_heads, dim].
 
     query [sequences, q_heads, dim]; q_heads is a multiple of the pools' heads and consecutive query heads share a KV head.
-    Sequence b attends its last `window` tokens (0 = all) of context_lens[b]; token t lies in page
-    block_table[b, t // page_tokens].  scale defaults to dim ** -0.5.  A sequence without tokens gives zeros.  What pages
+    Sequence b attends its last `window` slots (0 = all) of the context_lens[b] in use; slot t lies in page
+    block_table[b, t // page_tokens].  The last slots hold the last tokens as long as the cache is in order, that is, until
+    batch_evict_kv_pages first moves one; after it attend with window = 0.  A layer that looks back W tokens keeps just
+    those with budget = recent = W, evicting between append and attention.  scale defaults to dim ** -0.5.  A sequence without tokens gives zeros.  What pages
     hold behind a sequence's end never takes part, and neither do tokens on pages outside the pool; those pages, and
     lengths beyond the table (cut to it), are counted in `status`.
 
@@ -366,7 +368,8 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     as the heaviest).  With one weight head all KV heads keep the same tokens, else each head its own.  Survivors in
     slots from `budget` on move into the slots freed below it - rows of both pools, weight and position - so that
     the first `budget` slots hold what is kept, in no particular order, and the pages behind them are free.  The freed
-    slots get weight 0 and position -1.  Results go into `weights` and `positions` themselves unless `weights_out` or
+    slots get weight 0 and position -1.  Attention over what is left has no use for a window: it would go by slots, not by
+    positions.  Results go into `weights` and `positions` themselves unless `weights_out` or
     `positions_out` are given, which then receive every slot in use.
 
     Pages are packed in place: a page that two sequences share must be copied first.  A move from or to a page outside

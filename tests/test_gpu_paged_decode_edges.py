@@ -8,7 +8,8 @@ import paged_decode_oracle as oracle
 from test_gpu_paged_decode import DEV, _attend_case, _attend_tolerance
 
 from tair_kvcache_b200 import _cabi
-from tair_kvcache_b200.kernel import batch_append_kv_pages, batch_attend_kv_pages, rotary_frequencies
+from tair_kvcache_b200.kernel import (batch_append_kv_pages, batch_attend_kv_pages, batch_evict_kv_pages,
+                                      rotary_frequencies)
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +69,62 @@ def test_one_token_views_with_odd_strides():
         pools = torch.zeros_like(k_pool), torch.zeros_like(v_pool)
         results.append((batch_append_kv_pages(query, key, key, position, slot, *pools, inv_freq), *pools))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def _decode_loop(steps, batch, hq, hkv, dim, width, page, seed):
+    """Pools with room for two caches of the same sequences, and for each step the new tokens' queries, keys and values."""
+    gen = torch.Generator().manual_seed(seed)
+    pages = 2 * batch * width
+    pools = [torch.zeros(pages, page, hkv, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    tables = torch.randperm(pages, generator=gen).to(torch.int32).view(2, batch, width)
+    qkv = torch.randn(steps, batch, hq + 2 * hkv, dim, generator=gen).to(torch.bfloat16)
+    return pools, tables, qkv
+
+
+@pytest.mark.parametrize("hw", [1, 2])
+def test_a_cache_bounded_to_a_window_attends_what_the_window_does(hw):
+    """budget = recent = W and no window, against an unbounded cache in order and window W: the same tokens, so the same
+    attention - the tokens come in another order, so each within its own tolerance of the 64-bit form."""
+    steps, batch, hq, hkv, dim, width, page, w = 70, 2, 8, 2, 64, 10, 8, 21
+    (k_pool, v_pool), tables, qkv = _decode_loop(steps, batch, hq, hkv, dim, width, page, 3)
+    whole, bounded = tables.to(DEV)
+    inv_freq, _ = rotary_frequencies(dim, device=DEV)
+    lens = torch.zeros(batch, dtype=torch.int32, device=DEV)
+    weights = torch.zeros(batch, hw, width * page, device=DEV)
+    positions = torch.full((batch, hw, width * page), -1, dtype=torch.int32, device=DEV)
+    row = torch.arange(batch, device=DEV)
+    moved = False
+    for step in range(steps):
+        q, k, v = qkv[step].to(DEV).split([hq, hkv, hkv], dim=1)
+        at = torch.full((batch,), step, device=DEV)
+        batch_append_kv_pages(None, k, v, at, whole[row, at // page].long() * page + at % page, k_pool, v_pool, inv_freq)
+        to = lens.long()
+        q = batch_append_kv_pages(q, k, v, at, bounded[row, to // page].long() * page + to % page, k_pool, v_pool, inv_freq)
+        positions[row, :, to] = step
+        lens = batch_evict_kv_pages(k_pool, v_pool, bounded, lens + 1, weights, positions, w, recent=w)
+        got = batch_attend_kv_pages(q, k_pool, v_pool, bounded, lens, weights=weights)
+        windowed = batch_attend_kv_pages(q, k_pool, v_pool, whole, torch.full_like(lens, step + 1), window=w)
+        n = min(step + 1, w)
+        assert lens.tolist() == [n] * batch
+        assert (positions[..., :n].sort(dim=2).values == torch.arange(step + 1 - n, step + 1, device=DEV)).all()
+        moved = moved or not (positions[..., :n].diff(dim=2) == 1).all()
+        want, _, _, _, spread, size = oracle.attend(q.cpu(), k_pool.cpu(), v_pool.cpu(), tables[0],
+                                                    torch.full((batch,), step + 1), dim ** -0.5, w)
+        tol = _attend_tolerance(want, spread, size, w, "bf16")
+        for out in (got, windowed):
+            assert ((out.cpu().double() - want).abs() <= tol).all()
+    assert moved  # or there was nothing to tell apart
+
+
+def test_a_window_goes_by_slots_after_an_eviction():
+    """What the documentation says of a window over a cache that was evicted from: the last slots, whatever they hold."""
+    q, k_pool, v_pool, table, lens = _attend_case(9, [150, 90], 8, 2, 64, "bf16", poison=False)
+    dk, dv, dt = k_pool.to(DEV), v_pool.to(DEV), table.to(DEV)
+    weights = torch.rand(2, 2, table.shape[1] * 16, generator=torch.Generator().manual_seed(2)).to(DEV)
+    positions = torch.arange(weights.shape[2], dtype=torch.int32, device=DEV).expand_as(weights).contiguous()
+    new = batch_evict_kv_pages(dk, dv, dt, lens.to(DEV), weights, positions, 60, 10)
+    assert not (positions[0, 0, :60].diff() > 0).all()
+    for window in (0, 25):
+        want, _, _, _, spread, size = oracle.attend(q, dk.cpu(), dv.cpu(), table, new.cpu(), 0.125, window)
+        got = batch_attend_kv_pages(q.to(DEV), dk, dv, dt, new, window=window)
+        assert ((got.cpu().double() - want).abs() <= _attend_tolerance(want, spread, size, 60, "bf16")).all()
