@@ -989,7 +989,8 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
  * d_weights, when not NULL, accumulates the attention each cached token receives:
  *   weights_out[b][w][t] = weights[b][w][t] + sum over the query heads of KV head w of p_t     (n_weight_heads = n_kv_heads)
  *   weights_out[b][0][t] = weights[b][0][t] + sum over all query heads of p_t                  (n_weight_heads = 1)
- * for the attended t; other entries are left as they are.  The two may be the same memory with the same strides.
+ * for the t above; a token of them on a page outside the pool receives nothing, and its weight is carried over.  Entries of
+ * other t are left as they are.  The two may be the same memory with the same strides.
  * Strides of both, in elements, between sequences and between heads; every row has table_width * page_tokens entries.
  * Scores, softmax statistics, the sums and the weights are held in 32 bits; probabilities enter the product with V as
  * two 16-bit halves, so that only the output is rounded to 16 bits: they keep 16 bits in bf16, and in fp16 22 bits down

@@ -312,7 +312,8 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     lse: float32 [sequences, q_heads], receives the logarithm of the softmax sum (negative infinity without tokens).
     weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself) receives weights plus
     the attention each token got, summed over the query heads of its KV head or, with one weight head, over all of
-    them - what batch_evict_kv_pages ranks by.  Entries that are not attended are left as they are."""
+    them - what batch_evict_kv_pages ranks by.  A slot in the range whose page lies outside the pool gets its weight as it
+    was; entries out of the range are left as they are."""
     _no_grad(query, k_pool, v_pool, weights, out, lse, weights_out)
     pools, q_args, table_args, window, w_args, wo_args, size, default_scale, device = _attend_plan(
         int(window), out if out is None else _layout(out), lse if lse is None else _layout(lse),

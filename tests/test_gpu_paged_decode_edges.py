@@ -128,3 +128,30 @@ def test_a_window_goes_by_slots_after_an_eviction():
         want, _, _, _, spread, size = oracle.attend(q, dk.cpu(), dv.cpu(), table, new.cpu(), 0.125, window)
         got = batch_attend_kv_pages(q.to(DEV), dk, dv, dt, new, window=window)
         assert ((got.cpu().double() - want).abs() <= _attend_tolerance(want, spread, size, 60, "bf16")).all()
+
+
+@pytest.mark.parametrize("heads", ["kv", "one"])
+@pytest.mark.parametrize("window", [0, 100])
+def test_weights_of_bad_pages_are_carried_over(heads, window):
+    """With separate arrays: attended slots get old + received, slots of pages outside the pool their old weight, slots out of
+    the range nothing.  The bound is that of the accumulation's own test."""
+    lens = [170, 300, 64]
+    q, k_pool, v_pool, table, n = _attend_case(15, lens, 8, 2, 64, "bf16", poison=False)
+    table[0, 9], table[1, 4], table[1, 17], table[2, :4] = -1, k_pool.shape[0], 2 ** 31 - 1, -7
+    hw = 2 if heads == "kv" else 1
+    before = torch.rand(3, hw, table.shape[1] * 16, generator=torch.Generator().manual_seed(1))
+    out = torch.full_like(before, -3.0).to(DEV)
+    dk, dv = k_pool.to(DEV), v_pool.to(DEV)
+    batch_attend_kv_pages(q.to(DEV), dk, dv, table.to(DEV), n.to(DEV), window=window, weights=before.to(DEV), weights_out=out)
+    _, _, probs, firsts, _, size = oracle.attend(q, k_pool, v_pool, table, n, 0.125, window)
+    want, slack = torch.full(before.shape, -3.0, dtype=torch.float64), torch.zeros(before.shape, dtype=torch.float64)
+    for i, p in enumerate(probs):
+        t = slice(firsts[i], firsts[i] + p.shape[1])
+        mass = p.view(hw, 8 // hw, -1).sum(dim=1)
+        want[i, :, t] = before[i, :, t].double() + mass
+        slack[i, :, t] = mass * (2 * (2.0 ** -21 * size[i].max() + 2.0 ** -17) + 2.0 ** -18) + 2.0 ** -23 * want[i, :, t]
+    assert ((out.cpu().double() - want).abs() <= slack).all()
+    bad = (table < 0) | (table >= k_pool.shape[0])
+    for i, page in bad.nonzero().tolist():
+        t = [t for t in range(page * 16, page * 16 + 16) if firsts[i] <= t < lens[i]]
+        assert torch.equal(out[i, :, t].cpu(), before[i, :, t])
