@@ -1024,7 +1024,8 @@ KVCM_API int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const
  * new_lens[b] = min(len, budget).  Sequences with len <= budget keep everything.
  * weights_out / positions_out may be the input arrays with the same strides (the usual call) or other memory, which
  * then receives all slots below len; new_lens may not overlap context_lens.  Pages named by the kept part of two sequences at once (a shared prefix) would be
- * packed by both: copy them first.  Pages from ceil(budget / page_tokens) on are free afterwards.  A move from or to
+ * packed by both: copy them first.  Pages from ceil(budget / page_tokens) on are free afterwards; the others no
+ * longer hold the token blocks that their block hashes name, so they must not be stored or matched under those keys.  A move from or to
  * a page outside the pool is left out and counted; weight and position move all the same.  A length beyond
  * table_width * page_tokens is cut to it and counted.
  * 0 <= recent <= budget, budget >= 1.  d_workspace: kvcm_b200_evict_workspace_bytes, 16-byte aligned, contents irrelevant. */

@@ -373,7 +373,8 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     positions.  Results go into `weights` and `positions` themselves unless `weights_out` or
     `positions_out` are given, which then receive every slot in use.
 
-    Pages are packed in place: a page that two sequences share must be copied first.  A move from or to a page outside
+    Pages are packed in place: a page that two sequences share must be copied first, and an evicted page no longer holds the
+    tokens that its block hash names, so it must not be stored or matched under that key.  A move from or to a page outside
     the pool is left out and counted in `status`, as is a length beyond the table (cut to it)."""
     _no_grad(k_pool, v_pool, weights, weights_out)
     pools, table_args, batch, sizes, w_args, p_args, wo_args, po_args, size, device = _evict_plan(
