@@ -1017,7 +1017,8 @@ KVCM_API int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const
  * of which slot t holds the token of position positions[b][w][t] and weight weights[b][w][t]: when len > budget, the
  * `budget` slots that rank first are kept and packed into slots [0, budget).  Ranked first are the protected slots,
  * whose position is greater than (largest position in use) - recent; then by weight, larger first (NaN counts as the
- * largest); among equals the lower slot.  Survivors that lie below `budget` stay where they are; those above move, in
+ * largest); among equals the lower slot.  Protected slots are equals: positions that occur more than once can protect more
+ * slots than the budget holds, and the lower ones stay.  Survivors that lie below `budget` stay where they are; those above move, in
  * ascending order, into the freed slots below, in ascending order: K row, V row, weight and position (of KV head w, or
  * of all heads when n_weight_heads = 1).  Attention without a window does not depend on the order of slots, and
  * the positions array keeps every token's age.  Slots [budget, len) get weight 0 and position -1; slots from len on are left as they are.

@@ -366,7 +366,8 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     weights float32 and positions int32, both [sequences, 1 or kv_heads, >= table tokens]: of each slot in use the
     accumulated attention (batch_attend_kv_pages) and the position its token has in the text.  Kept are the tokens
     whose position is among the `recent` newest, then the heaviest; among equals the one in the lower slot (NaN counts
-    as the heaviest).  With one weight head all KV heads keep the same tokens, else each head its own.  Survivors in
+    as the heaviest).  Protected tokens are equals: where positions occur more than once and more of them are protected than
+    fit, those in the lower slots stay.  With one weight head all KV heads keep the same tokens, else each head its own.  Survivors in
     slots from `budget` on move into the slots freed below it - rows of both pools, weight and position - so that
     the first `budget` slots hold what is kept, in no particular order, and the pages behind them are free.  The freed
     slots get weight 0 and position -1.  Attention over what is left has no use for a window: it would go by slots, not by

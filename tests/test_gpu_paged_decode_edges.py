@@ -155,3 +155,33 @@ def test_weights_of_bad_pages_are_carried_over(heads, window):
     for i, page in bad.nonzero().tolist():
         t = [t for t in range(page * 16, page * 16 + 16) if firsts[i] <= t < lens[i]]
         assert torch.equal(out[i, :, t].cpu(), before[i, :, t])
+
+
+@pytest.mark.parametrize("tokens,budget,page", [(64, 10, 16), (5000, 700, 16), (400000, 20000, 64)])  # one CTA, a cluster, uncached
+def test_more_protected_slots_than_the_budget(tokens, budget, page):
+    """Positions that occur four times: more slots are protected than fit.  All of them rank equal, whatever their weights, so
+    the lowest stay; unprotected ones go, infinite and NaN weights among them."""
+    recent = budget // 2  # protects 4 * recent slots
+    gen = torch.Generator().manual_seed(tokens)
+    width = -(-tokens // page)
+    k_pool = torch.randn(width, page, 1, 8, generator=gen).to(torch.bfloat16)
+    v_pool = torch.randn(width, page, 1, 8, generator=gen).to(torch.bfloat16)
+    table = torch.arange(width, dtype=torch.int32)[None]
+    positions = torch.zeros(1, 1, width * page, dtype=torch.int32)
+    positions[0, 0, :tokens] = (torch.arange(tokens) // 4)[torch.randperm(tokens, generator=gen)].int()
+    weights = torch.rand(1, 1, width * page, generator=gen)
+    weights[0, 0, ::7], weights[0, 0, 3::11] = math.inf, math.nan
+    safe = positions[0, 0, :tokens] > positions[0, 0, :tokens].max() - recent
+    kept = safe.nonzero()[:budget, 0]
+    assert safe.sum() > budget
+    low = set(range(budget))
+    holes, movers = sorted(low - set(kept.tolist())), [t for t in kept.tolist() if t >= budget]
+    source = torch.arange(budget)
+    source[holes] = torch.tensor(movers)
+    dk, dv, dw, dp = k_pool.to(DEV), v_pool.to(DEV), weights.to(DEV), positions.to(DEV)
+    lens = batch_evict_kv_pages(dk, dv, table.to(DEV), torch.tensor([tokens], dtype=torch.int32, device=DEV), dw, dp, budget, recent)
+    assert lens.tolist() == [budget]
+    assert torch.equal(dp[0, 0, :budget].cpu(), positions[0, 0, source])
+    assert torch.equal(dw[0, 0, :budget].cpu().view(torch.int32), weights[0, 0, source].view(torch.int32))
+    for got, old in ((dk, k_pool), (dv, v_pool)):
+        assert torch.equal(got.cpu().view(-1, 8)[:budget].view(torch.int16), old.view(-1, 8)[source].view(torch.int16))
