@@ -984,7 +984,8 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
  * out is [batch][n_q_heads][head_dim] contiguous, of the pools' type; d_lse, when not NULL, receives the natural
  * logarithm of the softmax sum, [batch][n_q_heads].  A sequence without tokens, and a head whose scores are all
  * negative infinity, give zeros and an lse of negative infinity.  What lies behind a sequence's end in its last page,
- * or on pages it does not name, never takes part, NaN included.  A length beyond table_width * page_tokens is cut to
+ * or on pages it does not name, never takes part, NaN included.  An attended value that is not finite leaves that
+ * element of its heads' outputs not finite (infinite or NaN), other elements alone.  A length beyond table_width * page_tokens is cut to
  * it and counted; tokens on a page outside the pool take no part, and the page is counted.
  * d_weights, when not NULL, accumulates the attention each cached token receives:
  *   weights_out[b][w][t] = weights[b][w][t] + sum over the query heads of KV head w of p_t     (n_weight_heads = n_kv_heads)

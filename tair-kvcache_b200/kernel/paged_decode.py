@@ -306,7 +306,8 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     block_table[b, t // page_tokens].  The last slots hold the last tokens as long as the cache is in order, that is, until
     batch_evict_kv_pages first moves one; after it attend with window = 0.  A layer that looks back W tokens keeps just
     those with budget = recent = W, evicting between append and attention.  scale defaults to dim ** -0.5.  A sequence without tokens gives zeros.  What pages
-    hold behind a sequence's end never takes part, and neither do tokens on pages outside the pool; those pages, and
+    hold behind a sequence's end never takes part (an attended value that is infinite or NaN makes that element of the output
+    infinite or NaN), and neither do tokens on pages outside the pool; those pages, and
     lengths beyond the table (cut to it), are counted in `status`.
 
     lse: float32 [sequences, q_heads], receives the logarithm of the softmax sum (negative infinity without tokens).

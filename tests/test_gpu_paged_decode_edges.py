@@ -185,3 +185,25 @@ def test_more_protected_slots_than_the_budget(tokens, budget, page):
     assert torch.equal(dw[0, 0, :budget].cpu().view(torch.int32), weights[0, 0, source].view(torch.int32))
     for got, old in ((dk, k_pool), (dv, v_pool)):
         assert torch.equal(got.cpu().view(-1, 8)[:budget].view(torch.int16), old.view(-1, 8)[source].view(torch.int16))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (24, 2)])  # eight rows, sixteen
+@pytest.mark.parametrize("n", [50, 3000])              # whole, and cut and joined
+def test_attend_values_that_are_not_finite(n, hq, hkv, dtype):
+    """An element of an attended value that is infinite or NaN stays in its element and its KV head; one that is not
+    attended - before the window - is not seen at all."""
+    q, k_pool, v_pool, table, lens = _attend_case(n, [n], hq, hkv, 64, dtype, q_scale=0.5)
+    for t, head, element, value in ((n - 3, 0, 5, math.inf), (n - 20, 0, 6, -math.inf), (n - 7, 1, 7, math.nan), (n - 49, 0, 9, math.nan)):
+        v_pool[table[0, t // 16].long(), t % 16, head, element] = value
+    window = 40
+    got = batch_attend_kv_pages(q.to(DEV), k_pool.to(DEV), v_pool.to(DEV), table.to(DEV), lens.to(DEV), window=window).cpu()
+    finite = torch.ones(1, hq, 64, dtype=torch.bool)
+    finite[:, :hq // 2, 5:7] = False
+    finite[:, hq // 2:, 7] = False
+    assert torch.equal(got.isfinite(), finite)
+    want, _, _, _, spread, size = oracle.attend(q, k_pool, v_pool.nan_to_num(0.0, posinf=0.0, neginf=0.0), table, lens, 0.125, window)
+    assert ((got.double() - want).abs() <= _attend_tolerance(want, spread, size, window, dtype))[finite].all()
+    whole = batch_attend_kv_pages(q.to(DEV), k_pool.to(DEV), v_pool.to(DEV), table.to(DEV), lens.to(DEV)).cpu()
+    finite[:, :hq // 2, 9] = False  # the last one is attended now
+    assert torch.equal(whole.isfinite(), finite)
