@@ -181,13 +181,16 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 def _launch(name: str, device: torch.device, pools, *args) -> None:
+    """Both runtimes, torch's and the library's, have the pools' device current for the call, and torch's has its own back
+    afterwards: it is asked before the library's is changed, as the two share the driver's current context."""
     index = device.index
-    _cabi.bind_device(index)
     stream = _raw_stream(index)
     if torch.cuda.current_device() == index:
+        _cabi.bind_device(index)
         _cabi.call_pages(name, pools, *args, stream)
     else:
         with torch.cuda.device(device):
+            _cabi.bind_device(index)
             _cabi.call_pages(name, pools, *args, stream)
 
 

@@ -109,3 +109,35 @@ def test_strides_of_axes_of_length_one_say_nothing():
     assert attend_plan(k=k, v=v)[0][:4] == (1, 0, 128, 64)
     with pytest.raises(ValueError, match="one shape"):
         attend_plan(k=POOL, v=layout((10, 16, 2, 64), torch.bfloat16, (4096, 128, 64, 1)))
+
+
+def test_a_call_on_another_device_leaves_torchs_current_one(monkeypatch):
+    """The two runtimes share the driver's current context: whichever binds last is what both may report."""
+    current, events = [0], []
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.previous, current[0] = current[0], self.index
+            events.append(("torch", self.index))
+
+        def __exit__(self, *_):
+            current[0] = self.previous
+            events.append(("torch", self.previous))
+
+    def bind(index):
+        current[0] = index
+        events.append(("library", index))
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(paged_decode, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(_cabi, "bind_device", bind)
+    monkeypatch.setattr(_cabi, "call_pages", lambda name, pools, *args: events.append((name, current[0], args)))
+    paged_decode._launch("op", torch.device("cuda", 1), (), 7)
+    assert events == [("torch", 1), ("library", 1), ("op", 1, (7, 1001)), ("torch", 0)] and current == [0]
+    events.clear()
+    paged_decode._launch("op", torch.device("cuda", 0), (), 7)
+    assert events == [("library", 0), ("op", 0, (7, 1000))] and current == [0]
