@@ -958,7 +958,7 @@ typedef struct kvcm_b200_kv_pools {
  * `interleaved` - with cosine and sine multiplied by `attention_factor`; the rotated queries go to query_out, the
  * rotated keys and the values into token row slot_idx[t] of the pools.  Slot -1 marks a padding token: nothing is
  * written to the pools for it; any other slot outside the pool is skipped and counted.  Query and query_out may be the
- * same memory; key and value may not overlap the pools.  Angles are formed in 64 bits and reduced to one turn before
+ * same memory with the same strides, and otherwise may not overlap; key and value may not overlap the pools.  Angles are formed in 64 bits and reduced to one turn before
  * they are rounded, so positions of any magnitude an int32 holds keep their accuracy; products are formed in 32 bits
  * and rounded once.  A slot given twice is a data race, as in scatter.
  * d_query may be NULL with n_q_heads = 0.  Strides are in elements between tokens and between heads; elements of a head

@@ -300,6 +300,11 @@ int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
         addresses |= reinterpret_cast<uintptr_t>(d_query) | reinterpret_cast<uintptr_t>(d_query_out);
     }
     if (addresses & 1u) return KVCM_ER_INVALID_ADDRESS;
+    // A query that is rotated in place is read and written piece by piece, each by one thread.
+    if (n_q_heads > 0 && d_query == d_query_out && ((n_tokens > 1 && q_token_stride != qo_token_stride) ||
+                                                    (n_q_heads > 1 && q_head_stride != qo_head_stride))) {
+        return KVCM_ER_INVALID_PARAMS;
+    }
     if (!HaveDevice()) return KVCM_ER_NO_DEVICE;
     if (n_tokens == 0) return KVCM_OK;
     int v = 8;

@@ -158,7 +158,7 @@ def _sequences(table, lens, pool):
 
 def _per_slot(t, name: str, dtype: torch.dtype, pool, batch: int, tokens: int, heads=None):
     """Strides between sequences and heads, and the number of heads, of an array with an entry per slot."""
-    shape, strides = t[0], t[1]
+    shape, strides = t[0], _strides(t)
     if (len(shape) != 3 or t[2] != dtype or t[3] != pool[3] or shape[0] != batch or shape[2] < tokens or
             shape[1] not in ((1, pool[0][2]) if heads is None else (heads,)) or (strides[2] != 1 and shape[2] > 1)):
         raise ValueError("%s must be a %s [%d, %s, >= %d] tensor on the pools' device, contiguous along the last axis, "
@@ -243,7 +243,7 @@ def batch_append_kv_pages(query: Optional[torch.Tensor], key: torch.Tensor, valu
     `attention_factor`; the others pass through.  Token t's key and value go to pool token slot_indices[t] =
     page * page_tokens + offset, the numbers batch_scatter_kv_caches takes; -1 marks a padding token, which writes
     nothing; any other slot outside the pool is skipped and counted in `status` (four zeroed 32-bit words on the GPU).
-    The same slot twice in one call is a data race.  `query_out` may be `query`."""
+    The same slot twice in one call is a data race.  `query_out` may be `query`, or memory of its own."""
     _no_grad(query, key, value, inv_freq, k_pool, v_pool, query_out)
     if not isinstance(slot_indices, torch.Tensor):
         slot_indices = _index_tensor(slot_indices, k_pool.device)
@@ -314,7 +314,7 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     lengths beyond the table (cut to it), are counted in `status`.
 
     lse: float32 [sequences, q_heads], receives the logarithm of the softmax sum (negative infinity without tokens).
-    weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself) receives weights plus
+    weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself; else memory of its own) receives weights plus
     the attention each token got, summed over the query heads of its KV head or, with one weight head, over all of
     them - what batch_evict_kv_pages ranks by.  A slot in the range whose page lies outside the pool gets its weight as it
     was; entries out of the range are left as they are."""
@@ -376,7 +376,7 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     the first `budget` slots hold what is kept, in no particular order, and the pages behind them are free.  The freed
     slots get weight 0 and position -1.  Attention over what is left has no use for a window: it would go by slots, not by
     positions.  Results go into `weights` and `positions` themselves unless `weights_out` or
-    `positions_out` are given, which then receive every slot in use.
+    `positions_out` are given, memory of their own, which then receive every slot in use.
 
     Pages are packed in place: a page that two sequences share must be copied first, and an evicted page no longer holds the
     tokens that its block hash names, so it must not be stored or matched under that key.  A move from or to a page outside

@@ -141,3 +141,27 @@ def test_a_call_on_another_device_leaves_torchs_current_one(monkeypatch):
     events.clear()
     paged_decode._launch("op", torch.device("cuda", 0), (), 7)
     assert events == [("library", 0), ("op", 0, (7, 1000))] and current == [0]
+
+
+def test_same_memory_means_same_strides():
+    """In place is one layout twice.  A query and its result at one address with strides that differ where they count are
+    refused; where an axis has length one they do not count, for weights and positions neither."""
+    import ctypes
+    address = 1 << 20
+    pools = _cabi.KvPools(address, 2 * address, 10, 16 * 2 * 64, 2 * 64, 64, 16, 2, 64, _cabi.DTYPE_BF16)
+
+    def append(tokens, heads, strides, out_strides, out=address):
+        return _cabi.lib().kvcm_b200_append_pages(
+            ctypes.addressof(pools), address, *strides, heads, out, *out_strides, address, 128, 64, address, 128, 64, address, 8,
+            address, 4, tokens, address, 64, 0, 1.0, None, None)
+
+    if not torch.cuda.is_available():  # what passes the checks ends at the missing device
+        assert append(3, 4, (256, 64), (256, 64)) == _cabi.KVCM_ER_NO_DEVICE
+        assert append(1, 4, (256, 64), (512, 64)) == append(3, 1, (256, 64), (256, 128)) == _cabi.KVCM_ER_NO_DEVICE
+        assert append(3, 4, (256, 64), (512, 64), out=9 * address) == _cabi.KVCM_ER_NO_DEVICE
+    assert append(3, 4, (256, 64), (512, 64)) == append(3, 4, (256, 64), (64, 192)) == _cabi.KVCM_ER_INVALID_PARAMS
+    weights = layout((1, 1, 80), torch.float32, (80, 80, 1))
+    other = layout((1, 1, 80), torch.float32, (999, 77, 1))
+    plan = attend_plan(weights=weights, weights_out=other, query=layout((1, 4, 64), torch.bfloat16),
+                       table=layout((1, 5), torch.int32), lens=layout((1,), torch.int32))
+    assert plan[4] == plan[5] == (0, 0, 1)
