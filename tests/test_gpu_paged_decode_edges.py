@@ -1,10 +1,13 @@
 """The decode-step operators where numbers, shapes and callers are at their limits, against the 64-bit forms."""
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import paged_decode_oracle as oracle
+from conftest import ROOT
 from test_gpu_paged_decode import DEV, _attend_case, _attend_tolerance
 
 from tair_kvcache_b200 import _cabi
@@ -207,3 +210,48 @@ def test_attend_values_that_are_not_finite(n, hq, hkv, dtype):
     whole = batch_attend_kv_pages(q.to(DEV), k_pool.to(DEV), v_pool.to(DEV), table.to(DEV), lens.to(DEV)).cpu()
     finite[:, :hq // 2, 9] = False  # the last one is attended now
     assert torch.equal(whole.isfinite(), finite)
+
+
+_FIRST_CALL = """
+import sys
+sys.path.insert(0, %(root)r)
+import torch
+import tair_kvcache_b200
+from tair_kvcache_b200.kernel import batch_append_kv_pages, batch_attend_kv_pages, batch_evict_kv_pages, rotary_frequencies
+dev = torch.device("cuda:0")
+gen = torch.Generator().manual_seed(0)
+k, v = (torch.randn(%(pages)d, 16, 2, 64, generator=gen).to(torch.bfloat16).to(dev) for _ in range(2))
+qkv = torch.randn(1, 8, 64, generator=gen).to(torch.bfloat16).to(dev)
+table = torch.arange(%(pages)d, dtype=torch.int32, device=dev)[None]
+n = %(pages)d * 16
+lens = torch.tensor([n], dtype=torch.int32, device=dev)
+weights = torch.rand(1, 2, n, generator=gen).to(dev)
+positions = torch.arange(n, dtype=torch.int32).expand(1, 2, n).contiguous().to(dev)
+at = torch.tensor([n - 1], device=dev)
+inv_freq, _ = rotary_frequencies(64, device=dev)
+start = [t.clone() for t in (k, v, weights, positions)]
+
+def step():
+    q = batch_append_kv_pages(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], at, at, k, v, inv_freq)
+    out = batch_attend_kv_pages(q, k, v, table, lens, weights=weights)
+    return q, out, batch_evict_kv_pages(k, v, table, lens, weights, positions, n // 3, 5)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = step()
+graph.replay()
+first = [t.clone() for t in (*captured, k, v, weights, positions)]
+for t, old in zip((k, v, weights, positions), start):
+    t.copy_(old)
+assert all(torch.equal(a, b) for a, b in zip(first, (*step(), k, v, weights, positions)))
+print("captured first")
+"""
+
+
+@pytest.mark.parametrize("pages", [4, 2000])  # units whole, one CTA a head; cut and joined, a cluster of sixteen
+def test_the_first_call_of_a_process_may_be_captured(pages):
+    """Kernels, attributes and the device's answers are all met for the first time while a stream captures."""
+    proc = subprocess.run([sys.executable, "-c", _FIRST_CALL % dict(root=ROOT, pages=pages)], stdout=subprocess.PIPE,
+                          stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert proc.returncode == 0 and "captured first" in proc.stdout, proc.stdout[-2000:]
