@@ -963,8 +963,8 @@ typedef struct kvcm_b200_kv_pools {
  * and rounded once.  A slot given twice is a data race, as in scatter.
  * d_query may be NULL with n_q_heads = 0.  Strides are in elements between tokens and between heads; elements of a head
  * are contiguous.  position_bytes and slot_bytes say whether the index arrays hold 4- or 8-byte integers.  rotary_dim
- * is even, 0 .. head_dim <= 1024.  Fastest when all addresses and strides are multiples of 16 bytes and rotary_dim and head_dim - rotary_dim of 16 elements;
- * anything else is correct. */
+ * is even, 0 .. head_dim <= 1024.  Fastest when all addresses and strides are multiples of 16 bytes and rotary_dim and
+ * head_dim - rotary_dim of 16 elements; anything else is correct. */
 KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const void *d_query, int64_t q_token_stride,
                                         int64_t q_head_stride, int32_t n_q_heads, void *d_query_out,
                                         int64_t qo_token_stride, int64_t qo_head_stride, const void *d_key,
@@ -979,14 +979,16 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
  * [max(0, len - window), len), len = context_lens[b] (window 0 = all of them); slot t lies in page
  * block_table[b * table_stride + t / page_tokens].  A window goes by slots: it is the last tokens only while the cache is
  * in order, until kvcm_b200_evict_pages first moves one.  After that, window = 0; a layer that looks back W tokens keeps
- * them with budget = recent = W, evicting between append and attention.  Query head h reads KV head h / (n_q_heads / n_kv_heads):
+ * them with budget = recent = W, evicting between append and attention.  Query head h reads KV head
+ * h / (n_q_heads / n_kv_heads):
  *   out[b][h] = sum_t p_t V[t],  p = softmax(scale * query[b][h] . K[t])
  * out is [batch][n_q_heads][head_dim] contiguous, of the pools' type; d_lse, when not NULL, receives the natural
  * logarithm of the softmax sum, [batch][n_q_heads].  A sequence without tokens, and a head whose scores are all
  * negative infinity, give zeros and an lse of negative infinity.  What lies behind a sequence's end in its last page,
  * or on pages it does not name, never takes part, NaN included.  An attended value that is not finite leaves that
- * element of its heads' outputs not finite (infinite or NaN), other elements alone.  A length beyond table_width * page_tokens is cut to
- * it and counted; tokens on a page outside the pool take no part, and the page is counted.
+ * element of its heads' outputs not finite (infinite or NaN), other elements alone.  A length beyond
+ * table_width * page_tokens is cut to it and counted; tokens on a page outside the pool take no part, and the page is
+ * counted.
  * d_weights, when not NULL, accumulates the attention each cached token receives:
  *   weights_out[b][w][t] = weights[b][w][t] + sum over the query heads of KV head w of p_t     (n_weight_heads = n_kv_heads)
  *   weights_out[b][0][t] = weights[b][0][t] + sum over all query heads of p_t                  (n_weight_heads = 1)
@@ -997,9 +999,12 @@ KVCM_API int32_t kvcm_b200_append_pages(const kvcm_b200_kv_pools_t *pools, const
  * two 16-bit halves, so that only the output is rounded to 16 bits: they keep 16 bits in bf16, and in fp16 22 bits down
  * to 2^-28 of the largest of the head, with an error below 2^-40 of it.
  * The work is cut into equal shares over the GPU's SMs wherever sequences begin and end, so one long sequence uses all
- * of them; shares of one head are joined by a second kernel.  d_workspace holds the shares
- * (kvcm_b200_attend_workspace_bytes, 16-byte aligned, contents irrelevant); calls that may run at the same time need
- * separate workspaces.  Results do not depend on timing: the same inputs give the same bits.
+ * of them; shares of one head are joined by a second kernel.  d_workspace (kvcm_b200_attend_workspace_bytes, 16-byte
+ * aligned, contents irrelevant) holds the shares, 9 to 68 MB, and with weights the scores, 4 bytes for every sequence,
+ * query head and token of the table: its width counts, not the lengths, so pass no wider a table than the longest sequence
+ * needs.  Calls that may run at the same time need separate workspaces.  Results do not depend on timing: the same inputs
+ * give the same bits.
+ * A group of more than 16 query heads to a KV head reads that head's rows once per 16 of them.
  * head_dim is a multiple of 8, at most 256; pool addresses and strides are multiples of 16 bytes, query addresses and
  * strides of 4 bytes; at most 65,536 sequences, 4,096 query heads and 2^30 tokens of table per sequence, and 10^11
  * for batch * n_q_heads * (table tokens / 16 + 3). */
@@ -1019,17 +1024,17 @@ KVCM_API int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const
  * `budget` slots that rank first are kept and packed into slots [0, budget).  Ranked first are the protected slots,
  * whose position is greater than (largest position in use) - recent; then by weight, larger first (NaN counts as the
  * largest); among equals the lower slot.  Protected slots are equals: positions that occur more than once can protect more
- * slots than the budget holds, and the lower ones stay.  Survivors that lie below `budget` stay where they are; those above move, in
- * ascending order, into the freed slots below, in ascending order: K row, V row, weight and position (of KV head w, or
- * of all heads when n_weight_heads = 1).  Attention without a window does not depend on the order of slots, and
- * the positions array keeps every token's age.  Slots [budget, len) get weight 0 and position -1; slots from len on are left as they are.
- * new_lens[b] = min(len, budget).  Sequences with len <= budget keep everything.
+ * slots than the budget holds, and the lower ones stay.  Survivors that lie below `budget` stay where they are; those above
+ * move, in ascending order, into the freed slots below, in ascending order: K row, V row, weight and position (of KV head
+ * w, or of all heads when n_weight_heads = 1).  Attention without a window does not depend on the order of slots, and the
+ * positions array keeps every token's age.  Slots [budget, len) get weight 0 and position -1; slots from len on are left as
+ * they are.  new_lens[b] = min(len, budget).  Sequences with len <= budget keep everything.
  * weights_out / positions_out may be the input arrays with the same strides (the usual call) or other memory, which
- * then receives all slots below len; new_lens may not overlap context_lens.  Pages named by the kept part of two sequences at once (a shared prefix) would be
- * packed by both: copy them first.  Pages from ceil(budget / page_tokens) on are free afterwards; the others no
- * longer hold the token blocks that their block hashes name, so they must not be stored or matched under those keys.  A move from or to
- * a page outside the pool is left out and counted; weight and position move all the same.  A length beyond
- * table_width * page_tokens is cut to it and counted.
+ * then receives all slots below len; new_lens may not overlap context_lens.  Pages named by the kept part of two sequences
+ * at once (a shared prefix) would be packed by both: copy them first.  Pages from ceil(budget / page_tokens) on are free
+ * afterwards; the others no longer hold the token blocks that their block hashes name, so they must not be stored or
+ * matched under those keys.  A move from or to a page outside the pool is left out and counted; weight and position move
+ * all the same.  A length beyond table_width * page_tokens is cut to it and counted.
  * 0 <= recent <= budget, budget >= 1.  d_workspace: kvcm_b200_evict_workspace_bytes, 16-byte aligned, contents irrelevant. */
 KVCM_API int64_t kvcm_b200_evict_workspace_bytes(int32_t batch, int32_t n_weight_heads, int64_t table_tokens,
                                                  int32_t budget);

@@ -4,7 +4,9 @@
 //   o_h = sum_t p_t V[t],  p = softmax_t(scale * q_h . K[t]),  t over the sequence's last `window` tokens or all.
 //
 // Bound by HBM: every K and V row is read once (512 bytes per token and KV head of 128) and used by the query heads that
-// share the KV head, 2 to 32 multiplications per byte.  One pass with a running maximum and sum.
+// share the KV head, 2 to 32 multiplications per byte.  One pass with a running maximum and sum.  A group of more than
+// sixteen query heads is cut into row tiles of sixteen, each of which reads the rows again (groups of 17 and of 32 take
+// 2.2 and 2.3 times the time of one pass over the bytes, of 64 4.6 times).
 //
 // Four warps to a CTA, each with a ring of its own: tiles of 16 tokens of one KV head come from HBM by 16-byte asynchronous
 // copies, issued by the warp one to three tiles ahead, the table entry of the one after those already on its way; then
@@ -29,9 +31,9 @@
 // workspace, and the second kernel joins them, in order, so results do not depend on timing.  A third adds up the
 // weights, which need every head's final statistics.
 //
-// 64 sequences of 512 to 8192 tokens, 32 query and 8 KV heads of 128, bf16: 173 us, 6.6 TB/s, 101 % of a plain copy.  One
-// sequence of 131,072 tokens on one KV head: 21.6 us, of which 10.3 are its bytes; 16 of 2000 to 6001 tokens with weights:
-// 55 us, of which 41.
+// 64 sequences of 512 to 8192 tokens, 32 query and 8 KV heads of 128, bf16: 175 us, 6.5 TB/s read, as fast as a plain copy
+// reads and writes together.  One sequence of 131,072 tokens on one KV head, fp16: 22.5 us, of which 10.3 are its bytes; 16
+// of 2000 to 6001 tokens with weights: 55 us, of which 41.
 #include "paged_kv.cuh"
 
 namespace kvcm {
@@ -113,7 +115,7 @@ __device__ __forceinline__ int64_t PartAt(int32_t line, int32_t slot, int32_t wo
     return static_cast<int64_t>(line) * (2 * workers) + slot;
 }
 
-// Steps per run, the same in both kernels.
+// Steps per run, the same in the kernels that compute shares and join them.
 __device__ __forceinline__ int64_t StepsPerRun(int64_t all, int32_t workers) {
     const int64_t per = Divide(all + workers - 1, workers);
     return per > 1 ? per : 1;
@@ -1070,8 +1072,8 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.row_tiles = (group + rows - 1) / rows;
     // HBM and L2 move 64 to 256 bytes at a time.  Where a head's row is no multiple of 256 bytes and the next head's follows
     // it, a step takes rows of two or four heads instead of more tokens of one, so that what is fetched with a row is
-    // used: 177 -> 134 us for heads of 80 elements, 209 -> 183 us for 64; rows of 256 bytes take 174 us one head at a time
-    // and 175 to 177 us otherwise, as do pages that keep a head's tokens together.
+    // used: 177 -> 138 us for heads of 80 elements, 217 -> 198 us for 64, 181 -> 152 us for 96; rows of 256 bytes take 174 us
+    // one head at a time and 175 to 177 us otherwise, as do pages that keep a head's tokens together.
     p.step_heads = 1;
     const int32_t row_bytes = pools->head_dim * 2;
     if (pools->head_stride == pools->head_dim) {
@@ -1085,7 +1087,7 @@ int32_t kvcm_b200_attend_pages(const kvcm_b200_kv_pools_t *pools, const void *d_
     p.k_steps = (pools->head_dim + 15) / 16;
     p.v_minus_k = p.pools.v - p.pools.k;
     // A few steps are done sooner in one CTA than in several whose shares a second kernel joins: a table of
-    // kUncutSteps steps or less leaves every unit whole (one sequence of 100 tokens: 5.2 us instead of 7.5 us).
+    // kUncutSteps steps or less leaves every unit whole (one sequence of 100 tokens: 5.6 us instead of 7.3 us).
     p.uncut = table_tokens <= kUncutSteps * p.step_tokens;
     p.table_tokens = static_cast<int32_t>(table_tokens);
     p.window = window;

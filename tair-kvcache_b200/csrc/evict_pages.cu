@@ -14,7 +14,7 @@
 // packed by every SM.  (One kernel for both left the rows of a head to the cluster that ranked it: 703 us for 131,072
 // slots of eight heads instead of 59.)
 //
-// 128 heads of 6001 to 8192 slots cut to 4096, rows of 256 bytes: 18 us to rank, 45 us to move (5.4 TB/s read and
+// 128 heads of 6001 to 8192 slots cut to 4096, rows of 256 bytes: 64 us, 18 to rank, 45 to move (5.4 TB/s read and
 // written, 83 % of a plain copy: 256-byte rows scattered on both sides).  One sequence of 131,072 slots cut to 32,768, all
 // heads together: 23 us and 33 us (96 %).  256 heads one slot over their budget: 14 us together, a chain of latencies.
 // Counting with warp-wide matches instead of four copies of the counts took 29 and 61 us to rank the first two; reading
@@ -62,7 +62,6 @@ struct EvictParams {
     int64_t table_stride;
     int64_t w_batch, w_head, p_batch, p_head, wo_batch, wo_head, po_batch, po_head;
     int64_t max_moves;
-    int32_t table_width;
     int32_t table_tokens;
     int32_t n_heads;         // weight heads
     int32_t heads_per_move;  // KV heads that move together
@@ -577,7 +576,6 @@ int32_t kvcm_b200_evict_pages(const kvcm_b200_kv_pools_t *pools, int32_t batch, 
     p.po_batch = po_batch_stride;
     p.po_head = po_head_stride;
     p.max_moves = EvictMaxMoves(table_tokens, budget);
-    p.table_width = table_width;
     p.table_tokens = static_cast<int32_t>(table_tokens);
     p.n_heads = n_weight_heads;
     p.heads_per_move = n_weight_heads == 1 ? pools->n_kv_heads : 1;

@@ -308,16 +308,21 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     Sequence b attends its last `window` slots (0 = all) of the context_lens[b] in use; slot t lies in page
     block_table[b, t // page_tokens].  The last slots hold the last tokens as long as the cache is in order, that is, until
     batch_evict_kv_pages first moves one; after it attend with window = 0.  A layer that looks back W tokens keeps just
-    those with budget = recent = W, evicting between append and attention.  scale defaults to dim ** -0.5.  A sequence without tokens gives zeros.  What pages
-    hold behind a sequence's end never takes part (an attended value that is infinite or NaN makes that element of the output
-    infinite or NaN), and neither do tokens on pages outside the pool; those pages, and
-    lengths beyond the table (cut to it), are counted in `status`.
+    those with budget = recent = W, evicting between append and attention.  scale defaults to dim ** -0.5.  A sequence
+    without tokens gives zeros.  What pages hold behind a sequence's end never takes part, and neither do tokens on pages
+    outside the pool; those pages, and lengths beyond the table (cut to it), are counted in `status`.  An attended value that
+    is infinite or NaN makes that element of the output infinite or NaN.
 
     lse: float32 [sequences, q_heads], receives the logarithm of the softmax sum (negative infinity without tokens).
-    weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself; else memory of its own) receives weights plus
-    the attention each token got, summed over the query heads of its KV head or, with one weight head, over all of
-    them - what batch_evict_kv_pages ranks by.  A slot in the range whose page lies outside the pool gets its weight as it
-    was; entries out of the range are left as they are."""
+    weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself; else memory of its
+    own) receives weights plus the attention each token got, summed over the query heads of its KV head or, with one weight
+    head, over all of them - what batch_evict_kv_pages ranks by.  A slot in the range whose page lies outside the pool gets
+    its weight as it was; entries out of the range are left as they are.
+
+    Each call takes a workspace from torch: 9 to 68 MB for the shares of heads that several CTAs compute (17 MB for heads of
+    128 in groups of up to eight) and, with weights, 4 bytes per sequence, query head and token of the block table - of
+    the table's width, not of the lengths, which the host does not know.  256 sequences of 64 query heads with a table for
+    131,072 tokens take 8.6 GB: pass the part of the table that the longest sequence needs, block_table[:, :pages]."""
     _no_grad(query, k_pool, v_pool, weights, out, lse, weights_out)
     pools, q_args, table_args, window, w_args, wo_args, size, default_scale, device = _attend_plan(
         int(window), out if out is None else _layout(out), lse if lse is None else _layout(lse),
@@ -370,17 +375,17 @@ def batch_evict_kv_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table
     weights float32 and positions int32, both [sequences, 1 or kv_heads, >= table tokens]: of each slot in use the
     accumulated attention (batch_attend_kv_pages) and the position its token has in the text.  Kept are the tokens
     whose position is among the `recent` newest, then the heaviest; among equals the one in the lower slot (NaN counts
-    as the heaviest).  Protected tokens are equals: where positions occur more than once and more of them are protected than
-    fit, those in the lower slots stay.  With one weight head all KV heads keep the same tokens, else each head its own.  Survivors in
-    slots from `budget` on move into the slots freed below it - rows of both pools, weight and position - so that
-    the first `budget` slots hold what is kept, in no particular order, and the pages behind them are free.  The freed
-    slots get weight 0 and position -1.  Attention over what is left has no use for a window: it would go by slots, not by
-    positions.  Results go into `weights` and `positions` themselves unless `weights_out` or
-    `positions_out` are given, memory of their own, which then receive every slot in use.
+    as the heaviest).  Protected tokens are equals: where positions occur more than once and more of them are protected
+    than fit, those in the lower slots stay.  With one weight head all KV heads keep the same tokens, else each head its
+    own.  Survivors in slots from `budget` on move into the slots freed below it - rows of both pools, weight and position -
+    so that the first `budget` slots hold what is kept, in no particular order, and the pages behind them are free.  The
+    freed slots get weight 0 and position -1.  Attention over what is left has no use for a window: it would go by slots,
+    not by positions.  Results go into `weights` and `positions` themselves unless `weights_out` or `positions_out` are
+    given, memory of their own, which then receive every slot in use.
 
-    Pages are packed in place: a page that two sequences share must be copied first, and an evicted page no longer holds the
-    tokens that its block hash names, so it must not be stored or matched under that key.  A move from or to a page outside
-    the pool is left out and counted in `status`, as is a length beyond the table (cut to it)."""
+    Pages are packed in place: a page that two sequences share must be copied first, and an evicted page no longer holds
+    the tokens that its block hash names, so it must not be stored or matched under that key.  A move from or to a page
+    outside the pool is left out and counted in `status`, as is a length beyond the table (cut to it)."""
     _no_grad(k_pool, v_pool, weights, weights_out)
     pools, table_args, batch, sizes, w_args, p_args, wo_args, po_args, size, device = _evict_plan(
         int(budget), int(recent), weights_out if weights_out is None else _layout(weights_out),
