@@ -313,6 +313,7 @@ def batch_attend_kv_pages(query: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     outside the pool; those pages, and lengths beyond the table (cut to it), are counted in `status`.  An attended value that
     is infinite or NaN makes that element of the output infinite or NaN.
 
+    out (default: a new tensor): contiguous, of query's shape and type, memory of its own.
     lse: float32 [sequences, q_heads], receives the logarithm of the softmax sum (negative infinity without tokens).
     weights: float32 [sequences, 1 or kv_heads, >= table tokens]; weights_out (default: weights itself; else memory of its
     own) receives weights plus the attention each token got, summed over the query heads of its KV head or, with one weight

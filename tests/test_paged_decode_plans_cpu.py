@@ -165,3 +165,36 @@ def test_same_memory_means_same_strides():
     plan = attend_plan(weights=weights, weights_out=other, query=layout((1, 4, 64), torch.bfloat16),
                        table=layout((1, 5), torch.int32), lens=layout((1,), torch.int32))
     assert plan[4] == plan[5] == (0, 0, 1)
+
+
+@pytest.mark.parametrize("dim,base,factor,length", [(128, 10000.0, 8.0, 8192), (64, 500000.0, 32.0, 4096), (80, 10000.0, 3.5, 1000)])
+def test_the_inside_of_the_frequency_ramps(dim, base, factor, length):
+    """yarn and llama3 pair by pair from their definitions, in 64-bit numbers; float32 is off by half a step."""
+    def close(got, want):
+        return all(abs(g - w) <= w * (2.0 ** -24 + 1e-12) for g, w in zip(got.double().tolist(), want))
+
+    plain = [base ** (-2.0 * j / dim) for j in range(dim // 2)]
+    scaled, _ = paged_decode.rotary_frequencies(dim, base, "llama3", factor, length, device="cpu")
+    want, inside = [], 0
+    for f in plain:
+        wavelength = 2 * math.pi / f
+        if wavelength < length / 4.0:
+            want.append(f)
+        elif wavelength > length / 1.0:
+            want.append(f / factor)
+        else:
+            smooth = (length / wavelength - 1.0) / (4.0 - 1.0)
+            want.append((1 - smooth) * f / factor + smooth * f)
+            inside += 1
+    assert inside > 0 and close(scaled, want)
+    scaled, attention = paged_decode.rotary_frequencies(dim, base, "yarn", factor, length, device="cpu")
+
+    def pair(turns):  # the (real) pair whose angle makes that many turns over `length` tokens: base^(-2 j / dim) = 2 pi turns / length
+        return -dim / 2.0 * math.log(2 * math.pi * turns / length, base)
+
+    low, high = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), dim - 1)
+    want = []
+    for j, f in enumerate(plain):
+        share = min(max((j - low) / (high - low), 0.0), 1.0)  # of the interpolated frequency
+        want.append(f / factor * share + f * (1 - share))
+    assert high - low > 2 and close(scaled, want) and attention == 0.1 * math.log(factor) + 1.0
